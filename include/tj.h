@@ -313,6 +313,80 @@ TJ_API int tj_poly_attention_f16(const void* q, const void* k, const void* v, vo
                                  int batch, int heads, int seq_len, int exact_prefix, void* workspace,
                                  size_t workspace_bytes, int* err, void* stream);
 
+/* ---- training and 8-bit activations ------------------------------------- */
+
+typedef enum TjDtype { TJ_F32 = 0, TJ_F16 = 1, TJ_BF16 = 2, TJ_E4M3 = 3 } TjDtype;
+
+/* 8-bit tensors.  An activation [rows, cols] is e4m3 codes [rows, cols] and
+   one biased power-of-two exponent byte (e8m0) per row and run of 128
+   columns, scales [rows, ceil(cols/128)]; a weight [n, k] has one per 128 x
+   128 block, [ceil(n/128), ceil(k/128)].  With the block's largest finite
+   magnitude a the scale is the smallest 2^e, e >= -127, with a <= 448 * 2^e
+   (2^0 for zeros), and code = e4m3(value * 2^-e), to nearest even.
+   Infinities and NaN become the NaN code.  Packing is exact in the sense that
+   a block's codes depend on nothing but its values.
+   mask (nullable), in every entry below: one byte per row; rows with 0 are
+   not read, leave zeros in row-shaped outputs and nothing in sums.
+   None of these has a counterpart in the reference, which has no backward
+   pass and no 8-bit path; the forward arithmetic is that of nn.LayerNorm,
+   nn.Linear and the exact GELU (torch_transformer_benchmark.py:128-144). */
+TJ_API int tj_act8_pack(const void* x, int dtype, long long rows, int cols, const uint8_t* mask, void* codes,
+                        uint8_t* scales, void* stream);
+/* A value beyond the type's range becomes its largest one (65504 in 8 bits is
+   65536). */
+TJ_API int tj_act8_unpack(const void* codes, const uint8_t* scales, long long rows, int cols, void* out, int dtype,
+                          void* stream);
+/* transpose: codes [k, n] and scales [ceil(k/128), ceil(n/128)] of w's
+   transpose (the weight of the product that propagates a gradient back). */
+TJ_API int tj_weight8_pack(const void* w, int dtype, int n, int k, int transpose, void* codes, uint8_t* scales,
+                           void* stream);
+
+/* Layer norm that keeps its statistics: mean[rows], rstd[rows] (zeros for
+   masked rows).  y_dtype TJ_E4M3: y is codes, y_scales its scales (else
+   null).  x8_codes / x8_scales (nullable): also an 8-bit copy of x.
+   d <= 4096. */
+TJ_API int tj_layernorm_train(const void* x, int x_dtype, const float* gamma, const float* beta, long long rows, int d,
+                              float eps, const uint8_t* mask, void* y, int y_dtype, uint8_t* y_scales, float* mean,
+                              float* rstd, void* x8_codes, uint8_t* x8_scales, void* stream);
+TJ_API int tj_layernorm_backward_workspace_bytes(long long rows, int d, size_t* bytes);
+/* dx = rstd (g - sum(g)/d - xhat sum(g xhat)/d) [+ resid_grad], g = dy gamma,
+   xhat = (x - mean) rstd; dgamma, dbeta [d] are written (not added to).  x has
+   dx's type, or is 8-bit codes when x8_scales is given; resid_grad (nullable)
+   has dx's type and may alias dx.  Sums run in a fixed order. */
+TJ_API int tj_layernorm_backward(const void* dy, int dy_dtype, const void* x, const uint8_t* x8_scales,
+                                 const float* gamma, const float* mean, const float* rstd, long long rows, int d,
+                                 const uint8_t* mask, const void* resid_grad, void* dx, int dx_dtype, float* dgamma,
+                                 float* dbeta, void* workspace, size_t workspace_bytes, void* stream);
+
+/* dh = dy * gelu'(h) (exact GELU), of dy's type; h has dy's type, or is 8-bit
+   codes when h8_scales is given.  dh8_codes / dh8_scales (nullable): also the
+   8-bit form of the rounded dh. */
+TJ_API int tj_gelu_backward(const void* dy, int dtype, const void* h, const uint8_t* h8_scales, long long rows,
+                            int cols, const uint8_t* mask, void* dh, void* dh8_codes, uint8_t* dh8_scales,
+                            void* stream);
+
+/* out[m, n] = a[m, k] x w[n, k]^T [+ bias[n]] [+ resid[m, n]] on 8-bit
+   operands, FP32 sums; resid (FP32) only with out_dtype TJ_F32, and it may
+   alias out.  k % 16 == 0, n % 8 == 0.  err: an int that is zero, set to a
+   site code (401-404) when a bounded wait expires. */
+TJ_API int tj_gemm8(const void* a, const uint8_t* a_scales, const void* w, const uint8_t* w_scales, const float* bias,
+                    int m, int n, int k, const uint8_t* mask, const float* resid, void* out, int out_dtype, int* err,
+                    void* stream);
+/* h = a x w^T [+ bias]; writes g = gelu(h) and h, both in 8 bits (scales
+   [m, ceil(n/128)]).  n % 16 == 0. */
+TJ_API int tj_gemm8_gelu(const void* a, const uint8_t* a_scales, const void* w, const uint8_t* w_scales,
+                         const float* bias, int m, int n, int k, const uint8_t* mask, void* g_codes,
+                         uint8_t* g_scales, void* h_codes, uint8_t* h_scales, int* err, void* stream);
+
+TJ_API int tj_wgrad8_workspace_bytes(long long rows, int n, int k, size_t* bytes);
+/* dw[n, k] = dy[rows, n]^T x x[rows, k], db[n] = column sums of dy, written
+   (not added to).  dy is TJ_F16 or TJ_BF16; x is 8-bit and enters the product
+   restored to dy's type (exact in bf16; in fp16 as tj_act8_unpack).  n % 8 ==
+   0, k % 16 == 0.  Sums run in a fixed order.  err: as tj_gemm8 (501-504). */
+TJ_API int tj_wgrad8(const void* dy, int dtype, const void* x8_codes, const uint8_t* x8_scales, long long rows, int n,
+                     int k, const uint8_t* mask, float* dw, float* db, void* workspace, size_t workspace_bytes,
+                     int* err, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from ctypes import POINTER, c_char_p, c_float, c_int, c_size_t, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int, c_longlong, c_size_t, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().with_name("libtj.so")
@@ -18,6 +18,7 @@ TJ_ERR_DEVICE = 4
 STATUS_NAMES = {0: "TJ_OK", 1: "TJ_ERR_INVALID", 2: "TJ_ERR_UNSUPPORTED", 3: "TJ_ERR_CUDA",
                 4: "TJ_ERR_DEVICE", 5: "TJ_ERR_NO_DEVICE", 6: "TJ_ERR_NCCL"}
 ROUTE_EXACT, ROUTE_POLY, ROUTE_AUTO = 0, 1, 2
+F32, F16, BF16, E4M3 = 0, 1, 2, 3  # TjDtype
 EPI_QKV, EPI_GELU, EPI_RESID, EPI_PLAIN16 = 0, 1, 2, 3
 KERNEL_CLASSES = ("prep", "layernorm", "gemm_qkv", "attention", "gemm_out", "gemm_ffn_in", "gemm_ffn_out",
                   "layernorm_final", "poly")
@@ -86,6 +87,24 @@ SIGNATURES = {
                                       c_void_p, c_size_t, c_void_p, c_void_p]),
     "tj_attention_f16": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "tj_act8_pack": (c_int, [c_void_p, c_int, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "tj_act8_unpack": (c_int, [c_void_p, c_void_p, c_longlong, c_int, c_void_p, c_int, c_void_p]),
+    "tj_weight8_pack": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "tj_layernorm_train": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_longlong, c_int, c_float, c_void_p,
+                                   c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "tj_layernorm_backward_workspace_bytes": (c_int, [c_longlong, c_int, POINTER(c_size_t)]),
+    "tj_layernorm_backward": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong,
+                                      c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                      c_size_t, c_void_p]),
+    "tj_gelu_backward": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_void_p,
+                                 c_void_p, c_void_p]),
+    "tj_gemm8": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p,
+                         c_void_p, c_int, c_void_p, c_void_p]),
+    "tj_gemm8_gelu": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p,
+                              c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "tj_wgrad8_workspace_bytes": (c_int, [c_longlong, c_int, c_int, POINTER(c_size_t)]),
+    "tj_wgrad8": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                          c_void_p, c_size_t, c_void_p, c_void_p]),
 }
 
 _lock = threading.Lock()

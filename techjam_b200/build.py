@@ -12,12 +12,14 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libtj.so"
-SOURCES = ["tj_api.cu"]
+SOURCES = ["tj_api.cu", "tj_norm.cu", "tj_train.cu"]
+OBJ = PKG / "_build"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -29,7 +31,8 @@ def nvcc_path() -> str:
 
 
 def _inputs():
-    return [CSRC / s for s in SOURCES] + sorted(CSRC.glob("*.cuh")) + [PKG.parent / "include" / "tj.h"]
+    return [CSRC / s for s in SOURCES] + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [
+        PKG.parent / "include" / "tj.h"]
 
 
 def is_stale() -> bool:
@@ -43,16 +46,29 @@ def build(force: bool = False, verbose: bool = False, extra_flags=None) -> Path:
     """Compile ``libtj.so`` if any source is newer than it (or ``force``)."""
     if not force and not is_stale():
         return LIB
-    cmd = [nvcc_path(), *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
-           "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr", "-I", str(PKG.parent / "include"),
-           *(extra_flags or []), "-o", str(LIB) + ".tmp", *[str(CSRC / s) for s in SOURCES]]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stderr}\n{res.stdout}")
-    if verbose and res.stderr:
-        print(res.stderr, file=sys.stderr)
+    flags = [*ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler",
+             "-fvisibility=hidden", "--expt-relaxed-constexpr", "-I", str(PKG.parent / "include"),
+             *(extra_flags or [])]
+    OBJ.mkdir(exist_ok=True)
+    objects = [OBJ / (Path(s).stem + f".{os.getpid()}.o") for s in SOURCES]
+
+    def run(cmd):
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stderr}\n{res.stdout}")
+        if verbose and res.stderr:
+            print(res.stderr, file=sys.stderr)
+
+    try:
+        with ThreadPoolExecutor(len(SOURCES)) as pool:  # one nvcc per source, side by side
+            list(pool.map(lambda so: run([nvcc_path(), *flags, "-c", "-o", str(so[1]), str(CSRC / so[0])]),
+                          zip(SOURCES, objects)))
+        run([nvcc_path(), *ARCH_FLAGS, "-shared", "-o", str(LIB) + ".tmp", *map(str, objects)])
+    finally:
+        for o in objects:
+            o.unlink(missing_ok=True)
     os.replace(str(LIB) + ".tmp", LIB)
     return LIB
 

@@ -1,0 +1,377 @@
+// 8-bit activations: e4m3 codes with one power-of-two scale (e8m0) for each
+// run of 128 columns, and the memory-bound kernels on them (pack, restore,
+// weight pack, GELU's gradient).
+//
+// Of a block's finite values let a be the largest magnitude.  The scale is
+// the smallest 2^e, e >= -127, with a <= 448 * 2^e (448: e4m3's largest
+// value), 2^0 for a block of zeros, and code = e4m3(x * 2^-e), rounded to
+// nearest even.  The product x * 2^-e is exact (or far below half of e4m3's
+// smallest step), so a code depends on its block alone and is the same bit
+// for bit wherever the packing runs.  Infinities and NaN become the NaN code
+// and leave their neighbours' scale alone.  A power of two also keeps
+// code * 2^e exact in 32 bits and in bf16, and is what the tensor cores'
+// block-scaled products take.
+//
+// All kernels here move bytes once and are bound by HBM; a 128-column block
+// belongs to 8 lanes, so its maximum takes three shuffles, and the lanes'
+// 4-element pieces interleave so that every load and store of a warp covers
+// whole 32-byte sectors.
+#pragma once
+#include <cuda_bf16.h>
+
+#include <type_traits>
+
+#include "tj_common.cuh"
+
+namespace tj {
+
+constexpr int kBlk = 128;  // columns (and, for weights, rows) that share a scale
+
+enum Dtype : int { kF32 = 0, kF16 = 1, kBF16 = 2, kE4M3 = 3 };
+
+TJ_DEV int n_blocks(int cols) { return (cols + kBlk - 1) / kBlk; }
+
+// Biased exponent byte of the block scale for largest finite magnitude amax.
+// amax = 1.m * 2^(E-127); 448 = 1.75 * 2^8.
+TJ_DEV uint32_t scale_byte(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  if (u == 0u) return 127u;
+  const int b = (int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return (uint32_t)max(b, 0);
+}
+// 2^(127 - byte) for a byte that scale_byte gives (0..247): always normal.
+TJ_DEV float scale_inv(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+// 2^(byte - 127); 255 is NaN.
+TJ_DEV float scale_value(uint32_t byte) {
+  return __uint_as_float(byte == 0u ? 0x400000u : (byte == 255u ? 0x7fffffffu : byte << 23));
+}
+TJ_DEV float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a <= 3.402823466e38f ? a : 0.f;
+}
+// Codes of (a, b), a in the low byte.  x * 0 is NaN for an infinity or NaN,
+// which the conversion turns into the NaN code instead of saturating.
+TJ_DEV uint32_t e4m3x2(float a, float b, float inv) {
+  uint16_t r;
+  const float ya = fmaf(a, inv, a * 0.f), yb = fmaf(b, inv, b * 0.f);
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(yb), "f"(ya));
+  return r;
+}
+TJ_DEV uint32_t e4m3x4(const float (&v)[4], float inv) {
+  return e4m3x2(v[0], v[1], inv) | (e4m3x2(v[2], v[3], inv) << 16);
+}
+TJ_DEV void e4m3x4_value(uint32_t codes, float scale, float (&v)[4]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t f16;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(f16) : "h"((uint16_t)(codes >> (16 * h))));
+    const float2 f = __half22float2(*reinterpret_cast<__half2*>(&f16));
+    v[2 * h] = f.x * scale;
+    v[2 * h + 1] = f.y * scale;
+  }
+}
+
+// Four neighbouring elements of a row at column c (VEC: c + 3 < cols and the
+// address is aligned for one load; else element by element, zeros past cols).
+template <typename T>
+TJ_DEV float to_f32(T v);
+template <>
+TJ_DEV float to_f32<float>(float v) { return v; }
+template <>
+TJ_DEV float to_f32<__half>(__half v) { return __half2float(v); }
+template <>
+TJ_DEV float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// Rounded to nearest even.
+template <typename T>
+TJ_DEV T from_f32(float v);
+template <>
+TJ_DEV float from_f32<float>(float v) { return v; }
+template <>
+TJ_DEV __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+TJ_DEV __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+// A restored value: no infinity has a code, and one beyond T's range (a
+// rounded-up maximum: 65504 becomes 65536 in 8 bits) is T's largest.
+template <typename T>
+TJ_DEV T from_f32_restored(float v) {
+  constexpr float kMax = std::is_same_v<T, __half> ? 65504.f : (sizeof(T) == 2 ? 3.3895313892515355e38f : 3.402823466e38f);
+  if (fabsf(v) > kMax) v = copysignf(kMax, v);
+  return from_f32<T>(v);
+}
+
+template <typename T, bool VEC>
+TJ_DEV void load4(const T* row, int c, int cols, float (&v)[4]) {
+  if constexpr (VEC) {
+    if (c < cols) {
+      if constexpr (sizeof(T) == 4) {
+        const float4 f = *reinterpret_cast<const float4*>(row + c);
+        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+      } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(row + c);
+        const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = to_f32<T>(t[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = c + i < cols ? to_f32<T>(row[c + i]) : 0.f;
+  }
+}
+template <typename T, bool VEC>
+TJ_DEV void store4(T* row, int c, int cols, const T (&v)[4]) {
+  if constexpr (VEC) {
+    if (c < cols) {
+      if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(row + c) = make_float4(v[0], v[1], v[2], v[3]);
+      } else {
+        uint2 u;
+        T* t = reinterpret_cast<T*>(&u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = v[i];
+        *reinterpret_cast<uint2*>(row + c) = u;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i < cols) row[c + i] = v[i];
+  }
+}
+template <bool VEC>
+TJ_DEV uint32_t load_codes4(const uint8_t* row, int c, int cols) {
+  if constexpr (VEC) return c < cols ? *reinterpret_cast<const uint32_t*>(row + c) : 0u;
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (c + i < cols) w |= (uint32_t)row[c + i] << (8 * i);
+  return w;
+}
+template <bool VEC>
+TJ_DEV void store_codes4(uint8_t* row, int c, int cols, uint32_t w) {
+  if constexpr (VEC) {
+    if (c < cols) *reinterpret_cast<uint32_t*>(row + c) = w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i < cols) row[c + i] = (uint8_t)(w >> (8 * i));
+  }
+}
+
+// Largest over the 8 lanes that share a block.
+TJ_DEV float max8(float v) {
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// The 16 values of this lane (piece j: columns 4 * (lane%8 + 8 j) ..+3 of its
+// block at column c0) into codes, and the block's scale.  Called by whole warps.
+template <bool VEC>
+TJ_DEV void pack_block(const float (&v)[4][4], int c0, int cols, uint8_t* codes_row, uint8_t* scale, int sub,
+                       bool live) {
+  float amax = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) amax = fmaxf(amax, finite_abs(v[j][i]));
+  const uint32_t byte = scale_byte(max8(amax));
+  if (!live) return;
+  const float inv = scale_inv(byte);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) store_codes4<VEC>(codes_row, c0 + 4 * (sub + 8 * j), cols, e4m3x4(v[j], inv));
+  if (sub == 0) *scale = (uint8_t)byte;
+}
+
+// Block of this group of 8 lanes: four neighbouring blocks to a warp.
+struct BlockAt {
+  long long row;
+  int blk, c0;
+  bool live;
+};
+TJ_DEV BlockAt block_at(long long rows, int cols) {
+  const int nb = n_blocks(cols);
+  const long long g = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
+  BlockAt b;
+  b.live = g < rows * nb;
+  b.row = b.live ? g / nb : 0;
+  b.blk = b.live ? (int)(g - b.row * nb) : 0;
+  b.c0 = b.blk * kBlk;
+  return b;
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) act8_pack_kernel(const T* __restrict__ x, long long rows, int cols,
+                                                        const uint8_t* __restrict__ mask,
+                                                        uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  const BlockAt b = block_at(rows, cols);
+  const int sub = threadIdx.x & 7;
+  const bool valid = b.live && (mask == nullptr || mask[b.row] != 0);
+  float v[4][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) load4<T, VEC>(x + b.row * cols, b.c0 + 4 * (sub + 8 * j), valid ? cols : 0, v[j]);
+  pack_block<VEC>(v, b.c0, cols, codes + b.row * cols, scales + b.row * n_blocks(cols) + b.blk, sub, b.live);
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) act8_unpack_kernel(const uint8_t* __restrict__ codes,
+                                                          const uint8_t* __restrict__ scales, long long rows,
+                                                          int cols, T* __restrict__ out) {
+  const BlockAt b = block_at(rows, cols);
+  const int sub = threadIdx.x & 7;
+  if (!b.live) return;
+  const float s = scale_value(scales[b.row * n_blocks(cols) + b.blk]);
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = load_codes4<VEC>(codes + b.row * cols, b.c0 + 4 * (sub + 8 * j), cols);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float v[4];
+    e4m3x4_value(w[j], s, v);
+    T o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = from_f32_restored<T>(v[i]);
+    store4<T, VEC>(out + b.row * cols, b.c0 + 4 * (sub + 8 * j), cols, o);
+  }
+}
+
+// One CTA per 128 x 128 block of a weight [n, k]: codes [n, k] (or [k, n]
+// when TR) and one scale per block.  Runs when weights are loaded, not per
+// step; the transposed copy goes through shared memory.
+template <typename T, bool TR>
+__global__ void __launch_bounds__(256) weight8_pack_kernel(const T* __restrict__ w, int n, int k,
+                                                           uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  __shared__ float s_max[8];
+  __shared__ uint8_t s_codes[TR ? 128 * 129 : 1];
+  const int kb = blockIdx.x, nb = blockIdx.y;
+  const int col = kb * kBlk + (threadIdx.x & 127);
+  const int r0 = nb * kBlk + (threadIdx.x >> 7);
+  float amax = 0.f;
+  if (col < k)
+    for (int r = r0; r < min(n, (nb + 1) * kBlk); r += 2) amax = fmaxf(amax, finite_abs(to_f32<T>(w[(long long)r * k + col])));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = amax;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, s_max[i]);
+  const uint32_t byte = scale_byte(amax);
+  const float inv = scale_inv(byte);
+  if (threadIdx.x == 0) {
+    if constexpr (TR) scales[(long long)kb * n_blocks(n) + nb] = (uint8_t)byte;
+    else scales[(long long)nb * n_blocks(k) + kb] = (uint8_t)byte;
+  }
+  if (col < k)
+    for (int r = r0; r < min(n, (nb + 1) * kBlk); r += 2) {
+      const float v = to_f32<T>(w[(long long)r * k + col]);
+      const uint8_t c = (uint8_t)e4m3x2(v, 0.f, inv);
+      if constexpr (TR) s_codes[(threadIdx.x & 127) * 129 + (r - nb * kBlk)] = c;
+      else codes[(long long)r * k + col] = c;
+    }
+  if constexpr (TR) {
+    __syncthreads();
+    const int row = nb * kBlk + (threadIdx.x & 127);
+    if (row < n)
+      for (int c = threadIdx.x >> 7; c < min(kBlk, k - kb * kBlk); c += 2)
+        codes[(long long)(kb * kBlk + c) * n + row] = s_codes[c * 129 + (threadIdx.x & 127)];
+  }
+}
+
+// d gelu(h) / dh = Phi(h) + h phi(h), Phi the normal distribution and phi its
+// density, for the exact (erf) GELU.  With u = exp(-h^2 / 2),
+// phi = u / sqrt(2 pi) and, from Abramowitz & Stegun 7.1.26 (|error| 1.5e-7),
+// erfc(|h| / sqrt 2) = t q(t) u with t = 1 / (1 + p |h| / sqrt 2): one
+// exponential serves both terms, and for h < 0 nothing cancels.
+TJ_DEV float gelu_slope(float h) {
+  const float a = fabsf(h);
+  float t;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.3275911f * 0.70710678118654752f, a, 1.f)));
+  float q = fmaf(t, 1.061405429f, -1.453152027f);
+  q = fmaf(t, q, 1.421413741f);
+  q = fmaf(t, q, -0.284496736f);
+  q = fmaf(t, q, 0.254829592f);
+  // |h| > 1e18 would make h * h infinite times phi's zero
+  const float hc = fminf(fmaxf(h, -32.f), 32.f);
+  const float u = fast_exp2(hc * hc * -0.72134752044448170f);
+  const float half_erfc = 0.5f * t * q * u;
+  const float phi = 0.39894228040143268f * u;
+  const float s = fmaf(hc, phi, h >= 0.f ? 1.f - half_erfc : half_erfc);
+  return h == h ? s : h;  // fminf / fmaxf drop a NaN
+}
+
+// dh = dy * gelu'(h), rounded to T; PACK: also the 8-bit form of the rounded
+// dh, so that the packed copy is the one that packing dh would give.
+// h: 8-bit copy (H8) or a tensor of type T.
+template <typename T, bool H8, bool PACK, bool VEC>
+__global__ void __launch_bounds__(256) gelu_bwd_kernel(const T* __restrict__ dy, const void* __restrict__ h,
+                                                       const uint8_t* __restrict__ h_scales, long long rows, int cols,
+                                                       const uint8_t* __restrict__ mask, T* __restrict__ dh,
+                                                       uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  const BlockAt b = block_at(rows, cols);
+  const int sub = threadIdx.x & 7;
+  if (!PACK && !b.live) return;
+  const bool valid = b.live && (mask == nullptr || mask[b.row] != 0);
+  const int lim = valid ? cols : 0;
+  const long long base = b.row * cols;
+  float g[4][4], hv[4][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) load4<T, VEC>(dy + base, b.c0 + 4 * (sub + 8 * j), lim, g[j]);
+  if constexpr (H8) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      w[j] = load_codes4<VEC>(static_cast<const uint8_t*>(h) + base, b.c0 + 4 * (sub + 8 * j), lim);
+    const float s = valid ? scale_value(h_scales[b.row * n_blocks(cols) + b.blk]) : 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) e4m3x4_value(w[j], s, hv[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) load4<T, VEC>(static_cast<const T*>(h) + base, b.c0 + 4 * (sub + 8 * j), lim, hv[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    T o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o[i] = from_f32<T>(valid ? g[j][i] * gelu_slope(hv[j][i]) : 0.f);
+      if constexpr (PACK) g[j][i] = to_f32<T>(o[i]);
+    }
+    if (b.live) store4<T, VEC>(dh + base, b.c0 + 4 * (sub + 8 * j), cols, o);
+  }
+  if constexpr (PACK)
+    pack_block<VEC>(g, b.c0, cols, codes + base, scales + b.row * n_blocks(cols) + b.blk, sub, b.live);
+}
+
+// Column sums of in[n, cols], into out0 for c < split and out1 after it: 8 warps of a
+// CTA take every eighth row each and are joined in order.
+static __global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict__ in, int n, int cols,
+                                                          float* __restrict__ out0, float* __restrict__ out1,
+                                                          int split) {
+  __shared__ float s[8][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;
+  float a = 0.f;
+  if (c < cols) {
+    float b[4] = {0.f, 0.f, 0.f, 0.f};
+    int r = w;
+    for (; r + 24 < n; r += 32)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) b[q] += in[(size_t)(r + 8 * q) * cols + c];
+    for (; r < n; r += 8) b[0] += in[(size_t)r * cols + c];
+    a = (b[0] + b[1]) + (b[2] + b[3]);
+  }
+  s[w][lane] = a;
+  __syncthreads();
+  if (w == 0 && c < cols) {
+#pragma unroll
+    for (int q = 1; q < 8; ++q) a += s[q][lane];
+    if (c < split) out0[c] = a;
+    else out1[c - split] = a;
+  }
+}
+
+}  // namespace tj

@@ -16,6 +16,7 @@
 #include "tj_attention.cuh"
 #include "tj_common.cuh"
 #include "tj_gemm.cuh"
+#include "tj_host.h"
 #include "tj_misc.cuh"
 #include "tj_poly.cuh"
 
@@ -631,6 +632,47 @@ int launch_poly_route(const __half* q, const __half* k, const __half* v, __half*
 
 }  // namespace
 
+namespace tj_host {
+
+int fail(int status, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return ::fail(status, "%s", buf);
+}
+
+int device(int* index, int* sms) {
+  DeviceInfo di;
+  TJ_CHECK(device_info(&di));
+  TJ_CUDA(cudaGetDevice(index));
+  *sms = di.sms;
+  return TJ_OK;
+}
+
+int make_map(CUtensorMap* map, const void* base, int elt_bytes, uint64_t rows, uint64_t cols, uint32_t box_rows,
+             uint32_t box_cols) {
+  TJ_CHECK(get_encoder());
+  if ((reinterpret_cast<uintptr_t>(base) & 15) != 0) return ::fail(TJ_ERR_INVALID, "tensor base not 16-byte aligned");
+  if ((cols * elt_bytes) % 16 != 0)
+    return ::fail(TJ_ERR_UNSUPPORTED, "row pitch %llu bytes not a multiple of 16", (unsigned long long)(cols * elt_bytes));
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {cols * elt_bytes};
+  cuuint32_t box[2] = {box_cols, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapDataType type = elt_bytes == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : elt_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
+                                                    : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  CUresult r = g_encode(map, type, 2, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return ::fail(TJ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return TJ_OK;
+}
+
+}  // namespace tj_host
+
 extern "C" {
 
 int tj_version(void) { return 1; }
@@ -1017,7 +1059,7 @@ int tj_profile_end(TjModel* m, double* ms, long long* counts) {
 int tj_set_wait_limit(unsigned long long ns) {
   const unsigned long long v = ns == 0 ? TJ_WAIT_NS : ns;
   TJ_CUDA(cudaMemcpyToSymbol(tj::g_tj_wait_ns, &v, sizeof(v)));
-  return TJ_OK;
+  return tj_host::set_train_wait_limit(v);
 }
 
 int tj_set_pdl(int mode) {

@@ -22,7 +22,8 @@ namespace tj {
 
 // Limit of every bounded wait on this device, in ns of globaltimer time
 // (tj_set_wait_limit); read once by each wait that does not succeed at once.
-__device__ unsigned long long g_tj_wait_ns = TJ_WAIT_NS;
+// Each translation unit has its own copy; tj_set_wait_limit sets them all.
+static __device__ unsigned long long g_tj_wait_ns = TJ_WAIT_NS;
 
 // Error-site codes written to the device error word (first writer wins).
 enum ErrSite : int {
@@ -30,6 +31,8 @@ enum ErrSite : int {
   kErrGemmProducer = 101, kErrGemmMma = 102, kErrGemmEpilogue = 103,
   kErrAttnProducer = 201, kErrAttnMma = 202, kErrAttnSoftmax = 203,
   kErrPolyWait = 301,
+  kErrGemm8Producer = 401, kErrGemm8Mma = 402, kErrGemm8Scales = 403, kErrGemm8Epilogue = 404,
+  kErrWgradProducer = 501, kErrWgradMma = 502, kErrWgradRestore = 503, kErrWgradEpilogue = 504,
   kErrTest = 900,  // tj_wait_selftest: a wait that nothing completes
 };
 
@@ -87,6 +90,14 @@ TJ_DEV bool error_raised(const int* err) { return *reinterpret_cast<const volati
 // the warp stays converged for the elected tcgen05 issues that follow.
 TJ_DEV bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* err, int site) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, site));
+}
+// After an expired wait: the loads of a ring of n stages, issued up to (not
+// including) `stage` of pass `phase`, have landed (or the limit is reached)
+// before the thread goes on to leave the kernel.
+TJ_DEV void mbar_drain(uint64_t* full, int n, int stage, uint32_t phase) {
+  for (int i = 0; i < n; ++i)
+    for (int k = 0; k < (1 << 16) && !mbar_try_wait(full + i, i < stage ? phase : phase ^ 1u); ++k) {
+    }
 }
 // Plain arrive by one lane of a converged warp (barriers counting warps).
 TJ_DEV void mbar_arrive_elect(uint64_t* bar) {
