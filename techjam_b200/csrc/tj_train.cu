@@ -161,13 +161,13 @@ int wgrad_plan(long long rows, int n, int k, int sms, WgradPlan* w) {
   auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   w->list = 0;
   w->db = up(sizeof(int) * (size_t)(stages + 1));
-  w->dw = w->db + up(sizeof(float) * 2 * (size_t)n * w->splits * w->k_tiles);
+  w->dw = w->db + up(sizeof(float) * 4 * (size_t)n * w->splits * w->k_tiles);
   w->bytes = w->dw + (w->splits > 1 ? sizeof(float) * (size_t)n * k * w->splits : 0);
   return TJ_OK;
 }
 
 template <typename T>
-int launch_wgrad8(const void* dy, const tj::Wgrad8Params& p, int dev, int sms, cudaStream_t st) {
+int launch_wgrad8(const void* dy, const void* codes, const tj::Wgrad8Params& p, int dev, int sms, cudaStream_t st) {
   auto kern = tj::wgrad8_kernel<T>;
   static std::mutex mu;
   static int max_pairs[64] = {};
@@ -187,8 +187,8 @@ int launch_wgrad8(const void* dy, const tj::Wgrad8Params& p, int dev, int sms, c
     std::lock_guard<std::mutex> lock(mu);
     if (dev < 0 || dev >= 64) return fail(TJ_ERR_NO_DEVICE, "device index %d out of range", dev);
     if (max_pairs[dev] == 0) {
-      // The warpgroups' register budgets (48 + 112 + 2 * 176) add up to the
-      // launch's 4 * 128; with any other count an increase would wait for
+      // The warpgroups' register budgets (32 + 2 * 64 + 2 * 160) add up to the
+      // launch's 5 * 96; with any other count an increase would wait for
       // registers that nobody frees, so refuse to launch.
       cudaFuncAttributes fa;
       TJH_CUDA(cudaFuncGetAttributes(&fa, kern));
@@ -202,11 +202,12 @@ int launch_wgrad8(const void* dy, const tj::Wgrad8Params& p, int dev, int sms, c
     }
     pairs = max_pairs[dev];
   }
-  CUtensorMap ty;
+  CUtensorMap ty, tx;
   TJH_CHECK(tj_host::make_map(&ty, dy, 2, p.T, p.N, tj::kWgTok, 64));
+  TJH_CHECK(tj_host::make_map(&tx, codes, 1, p.T, p.K, tj::kWgTok, tj::kBlk));
   const long long items = (long long)((p.N + 255) / 256) * ((p.K + 255) / 256) * p.splits;
   cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(items, pairs));
-  TJH_CUDA(cudaLaunchKernelEx(&cfg, kern, ty, p));
+  TJH_CUDA(cudaLaunchKernelEx(&cfg, kern, ty, tx, p));
   return TJ_OK;
 }
 
@@ -357,7 +358,6 @@ int tj_wgrad8(const void* dy, int dtype, const void* x8_codes, const uint8_t* x8
   uint8_t* base = static_cast<uint8_t*>(workspace);
   tj::Wgrad8Params p{};
   p.T = rows; p.N = n; p.K = k;
-  p.codes = static_cast<const uint8_t*>(x8_codes);
   p.scales = x8_scales;
   p.mask = mask;
   p.splits = w.splits;
@@ -371,13 +371,14 @@ int tj_wgrad8(const void* dy, int dtype, const void* x8_codes, const uint8_t* x8
     p.list = list + 1;
     p.n_list = list;
   }
-  TJH_CHECK(dtype == TJ_F16 ? launch_wgrad8<__half>(dy, p, dev, sms, st) : launch_wgrad8<__nv_bfloat16>(dy, p, dev, sms, st));
+  TJH_CHECK(dtype == TJ_F16 ? launch_wgrad8<__half>(dy, x8_codes, p, dev, sms, st)
+                             : launch_wgrad8<__nv_bfloat16>(dy, x8_codes, p, dev, sms, st));
   if (w.splits > 1) {
     const long long total = (long long)n * k;
     tj::wgrad8_join_kernel<<<(unsigned)((total / 4 + 255) / 256), 256, 0, st>>>(p.dw, w.splits, total, dw);
     TJH_CUDA(cudaGetLastError());
   }
-  tj::column_sum_kernel<<<(n + 31) / 32, 256, 0, st>>>(p.db, 2 * w.splits * w.k_tiles, n, db, db, n);
+  tj::column_sum_kernel<<<(n + 31) / 32, 256, 0, st>>>(p.db, 4 * w.splits * w.k_tiles, n, db, db, n);
   TJH_CUDA(cudaGetLastError());
   return TJ_OK;
 }
