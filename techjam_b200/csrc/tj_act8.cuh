@@ -220,14 +220,17 @@ __global__ void __launch_bounds__(256) act8_pack_kernel(const T* __restrict__ x,
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) act8_unpack_kernel(const uint8_t* __restrict__ codes,
                                                           const uint8_t* __restrict__ scales, long long rows,
-                                                          int cols, T* __restrict__ out) {
+                                                          int cols, const uint8_t* __restrict__ mask,
+                                                          T* __restrict__ out) {
   const BlockAt b = block_at(rows, cols);
   const int sub = threadIdx.x & 7;
   if (!b.live) return;
-  const float s = scale_value(scales[b.row * n_blocks(cols) + b.blk]);
+  const bool valid = mask == nullptr || mask[b.row] != 0;
+  const float s = valid ? scale_value(scales[b.row * n_blocks(cols) + b.blk]) : 0.f;
   uint32_t w[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) w[j] = load_codes4<VEC>(codes + b.row * cols, b.c0 + 4 * (sub + 8 * j), cols);
+  for (int j = 0; j < 4; ++j)
+    w[j] = load_codes4<VEC>(codes + b.row * cols, b.c0 + 4 * (sub + 8 * j), valid ? cols : 0);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     float v[4];

@@ -32,7 +32,7 @@ enum ErrSite : int {
   kErrAttnProducer = 201, kErrAttnMma = 202, kErrAttnSoftmax = 203,
   kErrPolyWait = 301,
   kErrGemm8Producer = 401, kErrGemm8Mma = 402, kErrGemm8Scales = 403, kErrGemm8Epilogue = 404,
-  kErrWgradProducer = 501, kErrWgradMma = 502, kErrWgradRestore = 503, kErrWgradEpilogue = 504,
+  kErrWgradProducer = 501, kErrWgradMma = 502, kErrWgradEdge = 503, kErrWgradEpilogue = 504,
   kErrTest = 900,  // tj_wait_selftest: a wait that nothing completes
 };
 

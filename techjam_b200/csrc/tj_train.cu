@@ -43,10 +43,10 @@ int pack_t(const void* x, long long rows, int cols, const uint8_t* mask, uint8_t
   return TJ_OK;
 }
 template <typename T>
-int unpack_t(const uint8_t* codes, const uint8_t* scales, long long rows, int cols, void* out, bool vec,
-             unsigned grid, cudaStream_t st) {
-  if (vec) tj::act8_unpack_kernel<T, true><<<grid, 256, 0, st>>>(codes, scales, rows, cols, static_cast<T*>(out));
-  else tj::act8_unpack_kernel<T, false><<<grid, 256, 0, st>>>(codes, scales, rows, cols, static_cast<T*>(out));
+int unpack_t(const uint8_t* codes, const uint8_t* scales, long long rows, int cols, const uint8_t* mask, void* out,
+             bool vec, unsigned grid, cudaStream_t st) {
+  if (vec) tj::act8_unpack_kernel<T, true><<<grid, 256, 0, st>>>(codes, scales, rows, cols, mask, static_cast<T*>(out));
+  else tj::act8_unpack_kernel<T, false><<<grid, 256, 0, st>>>(codes, scales, rows, cols, mask, static_cast<T*>(out));
   TJH_CUDA(cudaGetLastError());
   return TJ_OK;
 }
@@ -146,7 +146,7 @@ int gemm8_kind(const Gemm8Args& g, const tj::Gemm8Params& p, int dev, int sms, c
 
 struct WgradPlan {
   int splits, k_tiles;
-  size_t list, db, dw, bytes;  // offsets of the stage list, the db parts and the dW parts
+  size_t list, db, x, dw, bytes;  // offsets of the stage list, the db parts, the restored input and the dW parts
 };
 int wgrad_plan(long long rows, int n, int k, int sms, WgradPlan* w) {
   if (rows < 0 || n <= 0 || k <= 0) return fail(TJ_ERR_INVALID, "weight gradient of [%lld, %d] and [%lld, %d]", rows, n, rows, k);
@@ -161,13 +161,14 @@ int wgrad_plan(long long rows, int n, int k, int sms, WgradPlan* w) {
   auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   w->list = 0;
   w->db = up(sizeof(int) * (size_t)(stages + 1));
-  w->dw = w->db + up(sizeof(float) * 4 * (size_t)n * w->splits * w->k_tiles);
+  w->x = w->db + up(sizeof(float) * 4 * (size_t)n * w->splits * w->k_tiles);
+  w->dw = w->x + up(2 * (size_t)rows * (size_t)k);
   w->bytes = w->dw + (w->splits > 1 ? sizeof(float) * (size_t)n * k * w->splits : 0);
   return TJ_OK;
 }
 
 template <typename T>
-int launch_wgrad8(const void* dy, const void* codes, const tj::Wgrad8Params& p, int dev, int sms, cudaStream_t st) {
+int launch_wgrad8(const void* dy, const void* x, const tj::Wgrad8Params& p, int dev, int sms, cudaStream_t st) {
   auto kern = tj::wgrad8_kernel<T>;
   static std::mutex mu;
   static int max_pairs[64] = {};
@@ -187,8 +188,8 @@ int launch_wgrad8(const void* dy, const void* codes, const tj::Wgrad8Params& p, 
     std::lock_guard<std::mutex> lock(mu);
     if (dev < 0 || dev >= 64) return fail(TJ_ERR_NO_DEVICE, "device index %d out of range", dev);
     if (max_pairs[dev] == 0) {
-      // The warpgroups' register budgets (32 + 2 * 64 + 2 * 160) add up to the
-      // launch's 5 * 96; with any other count an increase would wait for
+      // The warpgroups' register budgets (48 + 112 + 2 * 176) add up to the
+      // launch's 4 * 128; with any other count an increase would wait for
       // registers that nobody frees, so refuse to launch.
       cudaFuncAttributes fa;
       TJH_CUDA(cudaFuncGetAttributes(&fa, kern));
@@ -204,7 +205,7 @@ int launch_wgrad8(const void* dy, const void* codes, const tj::Wgrad8Params& p, 
   }
   CUtensorMap ty, tx;
   TJH_CHECK(tj_host::make_map(&ty, dy, 2, p.T, p.N, tj::kWgTok, 64));
-  TJH_CHECK(tj_host::make_map(&tx, codes, 1, p.T, p.K, tj::kWgTok, tj::kBlk));
+  TJH_CHECK(tj_host::make_map(&tx, x, 2, p.T, p.K, tj::kWgTok, 64));
   const long long items = (long long)((p.N + 255) / 256) * ((p.K + 255) / 256) * p.splits;
   cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(items, pairs));
   TJH_CUDA(cudaLaunchKernelEx(&cfg, kern, ty, tx, p));
@@ -243,9 +244,9 @@ int tj_act8_unpack(const void* codes, const uint8_t* scales, long long rows, int
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const uint8_t* c = static_cast<const uint8_t*>(codes);
   switch (dtype) {
-    case TJ_F32: return unpack_t<float>(c, scales, rows, cols, out, vec, grid, st);
-    case TJ_F16: return unpack_t<__half>(c, scales, rows, cols, out, vec, grid, st);
-    default: return unpack_t<__nv_bfloat16>(c, scales, rows, cols, out, vec, grid, st);
+    case TJ_F32: return unpack_t<float>(c, scales, rows, cols, nullptr, out, vec, grid, st);
+    case TJ_F16: return unpack_t<__half>(c, scales, rows, cols, nullptr, out, vec, grid, st);
+    default: return unpack_t<__nv_bfloat16>(c, scales, rows, cols, nullptr, out, vec, grid, st);
   }
 }
 
@@ -358,7 +359,7 @@ int tj_wgrad8(const void* dy, int dtype, const void* x8_codes, const uint8_t* x8
   uint8_t* base = static_cast<uint8_t*>(workspace);
   tj::Wgrad8Params p{};
   p.T = rows; p.N = n; p.K = k;
-  p.scales = x8_scales;
+  p.dy = dy;
   p.mask = mask;
   p.splits = w.splits;
   p.dw = w.splits > 1 ? reinterpret_cast<float*>(base + w.dw) : dw;
@@ -371,8 +372,16 @@ int tj_wgrad8(const void* dy, int dtype, const void* x8_codes, const uint8_t* x8
     p.list = list + 1;
     p.n_list = list;
   }
-  TJH_CHECK(dtype == TJ_F16 ? launch_wgrad8<__half>(dy, x8_codes, p, dev, sms, st)
-                             : launch_wgrad8<__nv_bfloat16>(dy, x8_codes, p, dev, sms, st));
+  unsigned grid;
+  TJH_CHECK(block_grid(rows, k, &grid));
+  const uint8_t* codes = static_cast<const uint8_t*>(x8_codes);
+  if (dtype == TJ_F16) {
+    TJH_CHECK(unpack_t<__half>(codes, x8_scales, rows, k, mask, base + w.x, true, grid, st));
+    TJH_CHECK(launch_wgrad8<__half>(dy, base + w.x, p, dev, sms, st));
+  } else {
+    TJH_CHECK(unpack_t<__nv_bfloat16>(codes, x8_scales, rows, k, mask, base + w.x, true, grid, st));
+    TJH_CHECK(launch_wgrad8<__nv_bfloat16>(dy, base + w.x, p, dev, sms, st));
+  }
   if (w.splits > 1) {
     const long long total = (long long)n * k;
     tj::wgrad8_join_kernel<<<(unsigned)((total / 4 + 255) / 256), 256, 0, st>>>(p.dw, w.splits, total, dw);
