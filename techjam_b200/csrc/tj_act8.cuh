@@ -49,16 +49,18 @@ TJ_DEV float finite_abs(float x) {
   const float a = fabsf(x);
   return a <= 3.402823466e38f ? a : 0.f;
 }
-// Codes of (a, b), a in the low byte.  x * 0 is NaN for an infinity or NaN,
-// which the conversion turns into the NaN code instead of saturating.
+// Codes of (a, b), a in the low byte.  The conversion saturates an infinity;
+// CAREFUL makes it the NaN code (x * 0 is NaN then).
+template <bool CAREFUL>
 TJ_DEV uint32_t e4m3x2(float a, float b, float inv) {
   uint16_t r;
-  const float ya = fmaf(a, inv, a * 0.f), yb = fmaf(b, inv, b * 0.f);
+  const float ya = CAREFUL ? fmaf(a, inv, a * 0.f) : a * inv, yb = CAREFUL ? fmaf(b, inv, b * 0.f) : b * inv;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(yb), "f"(ya));
   return r;
 }
+template <bool CAREFUL>
 TJ_DEV uint32_t e4m3x4(const float (&v)[4], float inv) {
-  return e4m3x2(v[0], v[1], inv) | (e4m3x2(v[2], v[3], inv) << 16);
+  return e4m3x2<CAREFUL>(v[0], v[1], inv) | (e4m3x2<CAREFUL>(v[2], v[3], inv) << 16);
 }
 TJ_DEV void e4m3x4_value(uint32_t codes, float scale, float (&v)[4]) {
 #pragma unroll
@@ -71,8 +73,15 @@ TJ_DEV void e4m3x4_value(uint32_t codes, float scale, float (&v)[4]) {
   }
 }
 
-// Four neighbouring elements of a row at column c (VEC: c + 3 < cols and the
-// address is aligned for one load; else element by element, zeros past cols).
+// A lane's share of a 128-column block at column c0: four pieces of four
+// elements.  VEC: piece j is columns 4 (sub + 8 j)..+3, one load (rows
+// aligned, widths a multiple of 4).  Otherwise element e of piece j is column
+// sub + 8 (4 j + e), so that the lanes' single-element accesses still lie
+// side by side.  Elements past cols read as zero and are not written.
+template <bool VEC>
+TJ_DEV int piece_col(int c0, int sub, int j, int e) {
+  return VEC ? c0 + 4 * (sub + 8 * j) + e : c0 + sub + 8 * (4 * j + e);
+}
 template <typename T>
 TJ_DEV float to_f32(T v);
 template <>
@@ -101,8 +110,9 @@ TJ_DEV T from_f32_restored(float v) {
 }
 
 template <typename T, bool VEC>
-TJ_DEV void load4(const T* row, int c, int cols, float (&v)[4]) {
+TJ_DEV void load4(const T* row, int c0, int sub, int j, int cols, float (&v)[4]) {
   if constexpr (VEC) {
+    const int c = piece_col<true>(c0, sub, j, 0);
     if (c < cols) {
       if constexpr (sizeof(T) == 4) {
         const float4 f = *reinterpret_cast<const float4*>(row + c);
@@ -119,12 +129,16 @@ TJ_DEV void load4(const T* row, int c, int cols, float (&v)[4]) {
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = c + i < cols ? to_f32<T>(row[c + i]) : 0.f;
+    for (int i = 0; i < 4; ++i) {
+      const int c = piece_col<false>(c0, sub, j, i);
+      v[i] = c < cols ? to_f32<T>(row[c]) : 0.f;
+    }
   }
 }
 template <typename T, bool VEC>
-TJ_DEV void store4(T* row, int c, int cols, const T (&v)[4]) {
+TJ_DEV void store4(T* row, int c0, int sub, int j, int cols, const T (&v)[4]) {
   if constexpr (VEC) {
+    const int c = piece_col<true>(c0, sub, j, 0);
     if (c < cols) {
       if constexpr (sizeof(T) == 4) {
         *reinterpret_cast<float4*>(row + c) = make_float4(v[0], v[1], v[2], v[3]);
@@ -138,28 +152,44 @@ TJ_DEV void store4(T* row, int c, int cols, const T (&v)[4]) {
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (c + i < cols) row[c + i] = v[i];
+    for (int i = 0; i < 4; ++i) {
+      const int c = piece_col<false>(c0, sub, j, i);
+      if (c < cols) row[c] = v[i];
+    }
   }
 }
 template <bool VEC>
-TJ_DEV uint32_t load_codes4(const uint8_t* row, int c, int cols) {
-  if constexpr (VEC) return c < cols ? *reinterpret_cast<const uint32_t*>(row + c) : 0u;
+TJ_DEV uint32_t load_codes4(const uint8_t* row, int c0, int sub, int j, int cols) {
+  if constexpr (VEC) {
+    const int c = piece_col<true>(c0, sub, j, 0);
+    return c < cols ? *reinterpret_cast<const uint32_t*>(row + c) : 0u;
+  }
   uint32_t w = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (c + i < cols) w |= (uint32_t)row[c + i] << (8 * i);
+  for (int i = 0; i < 4; ++i) {
+    const int c = piece_col<false>(c0, sub, j, i);
+    if (c < cols) w |= (uint32_t)row[c] << (8 * i);
+  }
   return w;
 }
 template <bool VEC>
-TJ_DEV void store_codes4(uint8_t* row, int c, int cols, uint32_t w) {
+TJ_DEV void store_codes4(uint8_t* row, int c0, int sub, int j, int cols, uint32_t w) {
   if constexpr (VEC) {
+    const int c = piece_col<true>(c0, sub, j, 0);
     if (c < cols) *reinterpret_cast<uint32_t*>(row + c) = w;
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (c + i < cols) row[c + i] = (uint8_t)(w >> (8 * i));
+    for (int i = 0; i < 4; ++i) {
+      const int c = piece_col<false>(c0, sub, j, i);
+      if (c < cols) row[c] = (uint8_t)(w >> (8 * i));
+    }
   }
+}
+
+TJ_DEV float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
 // Largest over the 8 lanes that share a block.
@@ -169,21 +199,36 @@ TJ_DEV float max8(float v) {
   return v;
 }
 
-// The 16 values of this lane (piece j: columns 4 * (lane%8 + 8 j) ..+3 of its
-// block at column c0) into codes, and the block's scale.  Called by whole warps.
+// The 16 values of this lane (its share of the block at column c0) into codes, and the block's scale.  Called by whole warps.
+// The maximum drops a NaN but not an infinity: only a warp that meets one
+// takes the finite values' maximum and the careful conversion.
 template <bool VEC>
 TJ_DEV void pack_block(const float (&v)[4][4], int c0, int cols, uint8_t* codes_row, uint8_t* scale, int sub,
                        bool live) {
   float amax = 0.f;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
+    amax = max3f(amax, fmaxf(fabsf(v[j][0]), fabsf(v[j][1])), fmaxf(fabsf(v[j][2]), fabsf(v[j][3])));
+  amax = max8(amax);
+  const bool careful = __any_sync(0xffffffffu, amax > 3.402823466e38f);
+  if (careful) {
+    amax = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) amax = fmaxf(amax, finite_abs(v[j][i]));
-  const uint32_t byte = scale_byte(max8(amax));
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) amax = fmaxf(amax, finite_abs(v[j][i]));
+    amax = max8(amax);
+  }
+  const uint32_t byte = scale_byte(amax);
   if (!live) return;
   const float inv = scale_inv(byte);
+  if (careful) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) store_codes4<VEC>(codes_row, c0 + 4 * (sub + 8 * j), cols, e4m3x4(v[j], inv));
+    for (int j = 0; j < 4; ++j) store_codes4<VEC>(codes_row, c0, sub, j, cols, e4m3x4<true>(v[j], inv));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) store_codes4<VEC>(codes_row, c0, sub, j, cols, e4m3x4<false>(v[j], inv));
+  }
   if (sub == 0) *scale = (uint8_t)byte;
 }
 
@@ -213,7 +258,7 @@ __global__ void __launch_bounds__(256) act8_pack_kernel(const T* __restrict__ x,
   const bool valid = b.live && (mask == nullptr || mask[b.row] != 0);
   float v[4][4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) load4<T, VEC>(x + b.row * cols, b.c0 + 4 * (sub + 8 * j), valid ? cols : 0, v[j]);
+  for (int j = 0; j < 4; ++j) load4<T, VEC>(x + b.row * cols, b.c0, sub, j, valid ? cols : 0, v[j]);
   pack_block<VEC>(v, b.c0, cols, codes + b.row * cols, scales + b.row * n_blocks(cols) + b.blk, sub, b.live);
 }
 
@@ -230,7 +275,7 @@ __global__ void __launch_bounds__(256) act8_unpack_kernel(const uint8_t* __restr
   uint32_t w[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j)
-    w[j] = load_codes4<VEC>(codes + b.row * cols, b.c0 + 4 * (sub + 8 * j), valid ? cols : 0);
+    w[j] = load_codes4<VEC>(codes + b.row * cols, b.c0, sub, j, valid ? cols : 0);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     float v[4];
@@ -238,7 +283,7 @@ __global__ void __launch_bounds__(256) act8_unpack_kernel(const uint8_t* __restr
     T o[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = from_f32_restored<T>(v[i]);
-    store4<T, VEC>(out + b.row * cols, b.c0 + 4 * (sub + 8 * j), cols, o);
+    store4<T, VEC>(out + b.row * cols, b.c0, sub, j, cols, o);
   }
 }
 
@@ -271,7 +316,7 @@ __global__ void __launch_bounds__(256) weight8_pack_kernel(const T* __restrict__
   if (col < k)
     for (int r = r0; r < min(n, (nb + 1) * kBlk); r += 2) {
       const float v = to_f32<T>(w[(long long)r * k + col]);
-      const uint8_t c = (uint8_t)e4m3x2(v, 0.f, inv);
+      const uint8_t c = (uint8_t)e4m3x2<true>(v, 0.f, inv);
       if constexpr (TR) s_codes[(threadIdx.x & 127) * 129 + (r - nb * kBlk)] = c;
       else codes[(long long)r * k + col] = c;
     }
@@ -285,25 +330,36 @@ __global__ void __launch_bounds__(256) weight8_pack_kernel(const T* __restrict__
 }
 
 // d gelu(h) / dh = Phi(h) + h phi(h), Phi the normal distribution and phi its
-// density, for the exact (erf) GELU.  With u = exp(-h^2 / 2),
-// phi = u / sqrt(2 pi) and, from Abramowitz & Stegun 7.1.26 (|error| 1.5e-7),
-// erfc(|h| / sqrt 2) = t q(t) u with t = 1 / (1 + p |h| / sqrt 2): one
-// exponential serves both terms, and for h < 0 nothing cancels.
-TJ_DEV float gelu_slope(float h) {
-  const float a = fabsf(h);
-  float t;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.3275911f * 0.70710678118654752f, a, 1.f)));
-  float q = fmaf(t, 1.061405429f, -1.453152027f);
-  q = fmaf(t, q, 1.421413741f);
-  q = fmaf(t, q, -0.284496736f);
-  q = fmaf(t, q, 0.254829592f);
-  // |h| > 1e18 would make h * h infinite times phi's zero
-  const float hc = fminf(fmaxf(h, -32.f), 32.f);
-  const float u = fast_exp2(hc * hc * -0.72134752044448170f);
-  const float half_erfc = 0.5f * t * q * u;
-  const float phi = 0.39894228040143268f * u;
-  const float s = fmaf(hc, phi, h >= 0.f ? 1.f - half_erfc : half_erfc);
-  return h == h ? s : h;  // fminf / fmaxf drop a NaN
+// density, for the exact (erf) GELU; two values at a time.  Odd about 1/2:
+// with a = |h| and u = exp(-a^2 / 2),
+//   slope = 1/2 + sign(h) (1/2 - erfc(a / sqrt 2) / 2 + a u / sqrt(2 pi)),
+// and from Abramowitz & Stegun 7.1.26 (|error| 1.5e-7) erfc(a / sqrt 2) =
+// t q(t) u, t = 1 / (1 + p a / sqrt 2): one exponential serves both terms.
+// z = a sqrt(log2(e) / 2) makes u = 2^(-z^2).  min.NaN keeps a NaN and makes
+// an infinity finite, so that a u is 0 and not NaN.  Four SFU operations for
+// two values (60 us of them at 32768 x 4096) hide behind the memory traffic.
+TJ_DEV float2 gelu_slope_x2(float h0, float h1) {
+  float a0, a1;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(a0) : "f"(fabsf(h0)), "f"(1e18f));
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(a1) : "f"(fabsf(h1)), "f"(1e18f));
+  constexpr float kZ = 0.84932180028801904f;                      // sqrt(log2(e) / 2)
+  constexpr float kP = 0.3275911f * 0.70710678118654752f / kZ;    // p / sqrt 2 in terms of z
+  constexpr float kPhi = 0.39894228040143268f / kZ;
+  const uint64_t z = fmul_x2(f32x2(a0, a1), f32x2(kZ, kZ));
+  const float2 den = f32x2_split(ffma_x2(z, f32x2(kP, kP), f32x2(1.f, 1.f)));
+  const float2 zz = f32x2_split(fmul_x2(z, z));
+  float t0, t1;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(den.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(den.y));
+  const uint64_t t = f32x2(t0, t1), u = f32x2(fast_exp2(-zz.x), fast_exp2(-zz.y));
+  // -q / 2, so that the sums below are plain fused multiply-adds
+  uint64_t q = ffma_x2(t, f32x2(-0.5f * 1.061405429f, -0.5f * 1.061405429f), f32x2(0.5f * 1.453152027f, 0.5f * 1.453152027f));
+  q = ffma_x2(t, q, f32x2(-0.5f * 1.421413741f, -0.5f * 1.421413741f));
+  q = ffma_x2(t, q, f32x2(0.5f * 0.284496736f, 0.5f * 0.284496736f));
+  q = ffma_x2(t, q, f32x2(-0.5f * 0.254829592f, -0.5f * 0.254829592f));
+  const uint64_t inner = ffma_x2(z, f32x2(kPhi, kPhi), fmul_x2(t, q));
+  const float2 m = f32x2_split(ffma_x2(u, inner, f32x2(0.5f, 0.5f)));
+  return make_float2(0.5f + copysignf(m.x, h0), 0.5f + copysignf(m.y, h1));
 }
 
 // dh = dy * gelu'(h), rounded to T; PACK: also the 8-bit form of the rounded
@@ -322,58 +378,68 @@ __global__ void __launch_bounds__(256) gelu_bwd_kernel(const T* __restrict__ dy,
   const long long base = b.row * cols;
   float g[4][4], hv[4][4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) load4<T, VEC>(dy + base, b.c0 + 4 * (sub + 8 * j), lim, g[j]);
+  for (int j = 0; j < 4; ++j) load4<T, VEC>(dy + base, b.c0, sub, j, lim, g[j]);
   if constexpr (H8) {
     uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      w[j] = load_codes4<VEC>(static_cast<const uint8_t*>(h) + base, b.c0 + 4 * (sub + 8 * j), lim);
+      w[j] = load_codes4<VEC>(static_cast<const uint8_t*>(h) + base, b.c0, sub, j, lim);
     const float s = valid ? scale_value(h_scales[b.row * n_blocks(cols) + b.blk]) : 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) e4m3x4_value(w[j], s, hv[j]);
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) load4<T, VEC>(static_cast<const T*>(h) + base, b.c0 + 4 * (sub + 8 * j), lim, hv[j]);
+    for (int j = 0; j < 4; ++j) load4<T, VEC>(static_cast<const T*>(h) + base, b.c0, sub, j, lim, hv[j]);
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     T o[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      o[i] = from_f32<T>(valid ? g[j][i] * gelu_slope(hv[j][i]) : 0.f);
-      if constexpr (PACK) g[j][i] = to_f32<T>(o[i]);
+    for (int i = 0; i < 4; i += 2) {
+      const float2 sl = gelu_slope_x2(hv[j][i], hv[j][i + 1]);
+      o[i] = from_f32<T>(g[j][i] * sl.x);  // masked rows: 0 * slope(0)
+      o[i + 1] = from_f32<T>(g[j][i + 1] * sl.y);
+      if constexpr (PACK) {
+        g[j][i] = to_f32<T>(o[i]);
+        g[j][i + 1] = to_f32<T>(o[i + 1]);
+      }
     }
-    if (b.live) store4<T, VEC>(dh + base, b.c0 + 4 * (sub + 8 * j), cols, o);
+    if (b.live) store4<T, VEC>(dh + base, b.c0, sub, j, cols, o);
   }
   if constexpr (PACK)
     pack_block<VEC>(g, b.c0, cols, codes + base, scales + b.row * n_blocks(cols) + b.blk, sub, b.live);
 }
 
-// Column sums of in[n, cols], into out0 for c < split and out1 after it: 8 warps of a
-// CTA take every eighth row each and are joined in order.
-static __global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict__ in, int n, int cols,
-                                                          float* __restrict__ out0, float* __restrict__ out1,
-                                                          int split) {
-  __shared__ float s[8][32];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;
+// Column sums of in[n, cols], into out0 for c < split and out1 after it: a CTA
+// has 8 columns (a 32-byte sector of a row), its 128 groups of 8 lanes every
+// 128th row each; joined in a fixed order.  (32 columns to a CTA: 7.6 us for
+// 592 x 2048, too few CTAs.)
+static __global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restrict__ in, int n, int cols,
+                                                                 float* __restrict__ out0, float* __restrict__ out1,
+                                                                 int split) {
+  __shared__ float s[128][9];
+  const int col = threadIdx.x & 7, grp = threadIdx.x >> 3;
+  const int c = blockIdx.x * 8 + col;
   float a = 0.f;
   if (c < cols) {
-    float b[4] = {0.f, 0.f, 0.f, 0.f};
-    int r = w;
-    for (; r + 24 < n; r += 32)
+    for (int r0 = grp; r0 < n; r0 += 128 * 8) {
+      float b[8];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) b[q] += in[(size_t)(r + 8 * q) * cols + c];
-    for (; r < n; r += 8) b[0] += in[(size_t)r * cols + c];
-    a = (b[0] + b[1]) + (b[2] + b[3]);
+      for (int q = 0; q < 8; ++q) b[q] = r0 + 128 * q < n ? in[(size_t)(r0 + 128 * q) * cols + c] : 0.f;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) a += b[q];
+    }
   }
-  s[w][lane] = a;
+  s[grp][col] = a;
   __syncthreads();
-  if (w == 0 && c < cols) {
-#pragma unroll
-    for (int q = 1; q < 8; ++q) a += s[q][lane];
-    if (c < split) out0[c] = a;
-    else out1[c - split] = a;
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (w < 8) {
+    const float t = warp_sum((s[lane][w] + s[lane + 32][w]) + (s[lane + 64][w] + s[lane + 96][w]));
+    const int cc = blockIdx.x * 8 + w;
+    if (lane == 0 && cc < cols) {
+      if (cc < split) out0[cc] = t;
+      else out1[cc - split] = t;
+    }
   }
 }
 

@@ -496,8 +496,8 @@ __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
                 const float2 g0 = gelu_erf_x2(h[4 * i], h[4 * i + 1]), g1 = gelu_erf_x2(h[4 * i + 2], h[4 * i + 3]);
-                gw[i] = e4m3x2(g0.x, g0.y, ginv) | (e4m3x2(g1.x, g1.y, ginv) << 16);
-                hw[i] = e4m3x2(h[4 * i], h[4 * i + 1], hinv) | (e4m3x2(h[4 * i + 2], h[4 * i + 3], hinv) << 16);
+                gw[i] = e4m3x2<true>(g0.x, g0.y, ginv) | (e4m3x2<true>(g1.x, g1.y, ginv) << 16);
+                hw[i] = e4m3x2<true>(h[4 * i], h[4 * i + 1], hinv) | (e4m3x2<true>(h[4 * i + 2], h[4 * i + 3], hinv) << 16);
               }
             }
           }

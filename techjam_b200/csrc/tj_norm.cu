@@ -51,41 +51,46 @@ int fwd_y(int y_dtype, const tj::NormFwdParams& p, bool vec, cudaStream_t st) {
   }
 }
 
-// CTAs of the backward pass for a width: a CTA holds kNormWarps / WR rows at a time.
-int bwd_grid(long long rows, int d, bool vec, int sms) {
-  const int wr = vec ? (d <= 1024 ? 1 : (d <= 2048 ? 2 : 4)) : (d <= 1024 ? 1 : 4);
-  const long long groups = tj::kNormWarps / wr;
-  return (int)std::max<long long>(1, std::min<long long>((rows + groups - 1) / groups, (long long)tj::kNormBwdCtas * sms));
+// Warps that share a row in the backward pass: 512 columns each.
+int bwd_wr(int d) { return d <= 512 ? 1 : (d <= 1024 ? 2 : (d <= 2048 ? 4 : 8)); }
+
+// CTAs of the backward pass: as many as run at once, at most one per row group.
+int bwd_grid(long long rows, int d, int sms) {
+  const int wr = bwd_wr(d), warps = tj::norm_bwd_warps(wr);
+  const long long groups = warps / wr;
+  return (int)std::max<long long>(1, std::min<long long>((rows + groups - 1) / groups, (long long)tj::norm_bwd_ctas(wr) * sms));
 }
 
-template <typename DY, typename X, bool X8>
-struct Bwd {
-  const tj::NormBwdParams& p;
-  int sms;
-  cudaStream_t st;
-  template <int WR, int NI, bool VEC>
-  int operator()() const {
-    const int grid = bwd_grid(p.rows, p.d, VEC, sms);
-    tj::norm_bwd_kernel<DY, X, X8, WR, NI, VEC><<<grid, 32 * tj::kNormWarps, 0, st>>>(p);
+template <typename DY, typename X, bool X8, int WR>
+int bwd_launch(const tj::NormBwdParams& p, bool vec, int sms, cudaStream_t st) {
+  const int grid = bwd_grid(p.rows, p.d, sms);
+  if (vec) tj::norm_bwd_kernel<DY, X, X8, WR, true><<<grid, 32 * tj::norm_bwd_warps(WR), 0, st>>>(p);
+  else tj::norm_bwd_kernel<DY, X, X8, WR, false><<<grid, 32 * tj::norm_bwd_warps(WR), 0, st>>>(p);
+  TJH_CUDA(cudaGetLastError());
+  if (grid > 1) {
+    tj::column_sum_kernel<<<(2 * p.d + 7) / 8, 1024, 0, st>>>(p.partial, grid, 2 * p.d, p.dgamma, p.dbeta, p.d);
     TJH_CUDA(cudaGetLastError());
-    if (grid > 1) {
-      tj::column_sum_kernel<<<(2 * p.d + 31) / 32, 256, 0, st>>>(p.partial, grid, 2 * p.d, p.dgamma, p.dbeta, p.d);
-      TJH_CUDA(cudaGetLastError());
-    }
-    return TJ_OK;
   }
-};
+  return TJ_OK;
+}
+template <typename DY, typename X, bool X8>
+int bwd_width(const tj::NormBwdParams& p, bool vec, int sms, cudaStream_t st) {
+  switch (bwd_wr(p.d)) {
+    case 1: return bwd_launch<DY, X, X8, 1>(p, vec, sms, st);
+    case 2: return bwd_launch<DY, X, X8, 2>(p, vec, sms, st);
+    case 4: return bwd_launch<DY, X, X8, 4>(p, vec, sms, st);
+    default: return bwd_launch<DY, X, X8, 8>(p, vec, sms, st);
+  }
+}
 
 template <typename DY>
 int bwd_x(int dx_dtype, bool x8, const tj::NormBwdParams& p, bool vec, int sms, cudaStream_t st) {
   switch (dx_dtype) {
-    case TJ_F32:
-      return x8 ? by_width(p.d, vec, Bwd<DY, float, true>{p, sms, st}) : by_width(p.d, vec, Bwd<DY, float, false>{p, sms, st});
-    case TJ_F16:
-      return x8 ? by_width(p.d, vec, Bwd<DY, __half, true>{p, sms, st}) : by_width(p.d, vec, Bwd<DY, __half, false>{p, sms, st});
+    case TJ_F32: return x8 ? bwd_width<DY, float, true>(p, vec, sms, st) : bwd_width<DY, float, false>(p, vec, sms, st);
+    case TJ_F16: return x8 ? bwd_width<DY, __half, true>(p, vec, sms, st) : bwd_width<DY, __half, false>(p, vec, sms, st);
     default:
-      return x8 ? by_width(p.d, vec, Bwd<DY, __nv_bfloat16, true>{p, sms, st})
-                : by_width(p.d, vec, Bwd<DY, __nv_bfloat16, false>{p, sms, st});
+      return x8 ? bwd_width<DY, __nv_bfloat16, true>(p, vec, sms, st)
+                : bwd_width<DY, __nv_bfloat16, false>(p, vec, sms, st);
   }
 }
 
@@ -128,7 +133,7 @@ int tj_layernorm_backward_workspace_bytes(long long rows, int d, size_t* bytes) 
   if (!bytes) return fail(TJ_ERR_INVALID, "null argument");
   int dev, sms;
   TJH_CHECK(tj_host::device(&dev, &sms));
-  const int grid = std::max(bwd_grid(rows, d, true, sms), bwd_grid(rows, d, false, sms));
+  const int grid = bwd_grid(rows, d, sms);
   *bytes = grid > 1 ? (size_t)grid * 2 * d * sizeof(float) : 0;
   return TJ_OK;
 }

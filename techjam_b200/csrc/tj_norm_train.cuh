@@ -8,9 +8,10 @@
 //   dgamma = sum over rows of dy * xhat,  dbeta = sum over rows of dy
 //
 // Bound by HBM: every row is read once and written once, and held in
-// registers in between.  WR warps share a row, each 1024 of its columns, so
-// that a row's x, dy and the lane's share of dgamma and dbeta stay within the
-// register file at every width.  Columns are laid out as in tj_act8.cuh: a
+// registers in between.  WR warps share a row: each has 1024 of its columns
+// forward, and 512 backward, where x, dy, the residual's gradient and the
+// lane's share of dgamma and dbeta take five registers a column (1024 a warp
+// spilled at 168 registers; see norm_bwd_kernel).  Columns are laid out as in tj_act8.cuh: a
 // 128-column block belongs to 8 lanes.  Rows whose mask byte is 0 are not
 // read: they leave zeros in every output and nothing in the sums.
 #pragma once
@@ -18,40 +19,42 @@
 
 namespace tj {
 
-// Column of element 0 of piece (i, j) of this lane within the warp's 1024 columns.
-TJ_DEV int norm_col(int lane, int i, int j) { return 512 * i + 128 * (lane >> 3) + 4 * ((lane & 7) + 8 * j); }
+// First column of this lane's block in step i of the warp's 1024 columns.
+TJ_DEV int norm_blk(int lane, int i) { return 512 * i + 128 * (lane >> 3); }
+// Column of element e of its piece j there.
+template <bool VEC>
+TJ_DEV int norm_col(int lane, int i, int j, int e) { return piece_col<VEC>(norm_blk(lane, i), lane & 7, j, e); }
 
-TJ_DEV float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-// Sum of N values over the WR warps of a row (whole CTA when WR > 1: its
-// rows run in step).  Every warp gets the same bits.
-template <int WR, int N>
-TJ_DEV void row_sum(float (&v)[N], float* smem, int warp, int lane) {
+// Sum of N values over the WR warps of a row, WARPS warps in the CTA, whose
+// rows run in step when WR > 1.  Every warp gets the same bits.  smem holds two
+// sets, used in turn (`turn` flips): with one barrier between, a set is
+// written again only after every warp has read it.
+template <int WARPS, int WR, int N>
+TJ_DEV void row_sum(float (&v)[N], float (*smem)[WARPS * N], int& turn, int warp, int lane) {
 #pragma unroll
   for (int n = 0; n < N; ++n) v[n] = warp_sum(v[n]);
   if constexpr (WR > 1) {
+    float* set = smem[turn];
+    turn ^= 1;
     if (lane == 0)
 #pragma unroll
-      for (int n = 0; n < N; ++n) smem[warp * N + n] = v[n];
+      for (int n = 0; n < N; ++n) set[warp * N + n] = v[n];
     __syncthreads();
     const int w0 = warp - warp % WR;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < WR; ++w) s += smem[(w0 + w) * N + n];
+      for (int w = 0; w < WR; ++w) s += set[(w0 + w) * N + n];
       v[n] = s;
     }
-    __syncthreads();
   }
 }
 
-constexpr int kNormWarps = 4;    // warps per CTA in both passes
-constexpr int kNormBwdCtas = 3;  // CTAs per SM in the backward pass
+constexpr int kNormWarps = 4;    // warps per CTA forward, and backward up to 2048 columns
+// Warps per CTA and CTAs per SM backward: 16 warps of up to 128 registers.
+constexpr int norm_bwd_warps(int wr) { return wr > kNormWarps ? wr : kNormWarps; }
+constexpr int norm_bwd_ctas(int wr) { return 16 / norm_bwd_warps(wr); }
 
 struct NormFwdParams {
   const void* x;
@@ -71,8 +74,9 @@ struct NormFwdParams {
 
 // NI: 512-column steps per warp (1 or 2).
 template <typename T, typename Y, int WR, int NI, bool VEC>
-__global__ void __launch_bounds__(32 * kNormWarps) norm_fwd_kernel(const NormFwdParams p) {
-  __shared__ float s_red[kNormWarps];
+__global__ void __launch_bounds__(32 * kNormWarps, 6) norm_fwd_kernel(const NormFwdParams p) {
+  __shared__ float s_red[2][kNormWarps];
+  int red = 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long row = (long long)blockIdx.x * (kNormWarps / WR) + warp / WR;
   const int base = (warp % WR) * 1024;
@@ -86,10 +90,10 @@ __global__ void __launch_bounds__(32 * kNormWarps) norm_fwd_kernel(const NormFwd
   for (int i = 0; i < NI; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      load4<T, VEC>(static_cast<const T*>(p.x) + at, base + norm_col(lane, i, j), lim, v[i][j]);
+      load4<T, VEC>(static_cast<const T*>(p.x) + at, base + norm_blk(lane, i), lane & 7, j, lim, v[i][j]);
       sum[0] += (v[i][j][0] + v[i][j][1]) + (v[i][j][2] + v[i][j][3]);
     }
-  row_sum<WR, 1>(sum, s_red, warp, lane);
+  row_sum<kNormWarps, WR, 1>(sum, s_red, red, warp, lane);
   const float mean = sum[0] / d;
   float sq[1] = {0.f};
 #pragma unroll
@@ -99,9 +103,9 @@ __global__ void __launch_bounds__(32 * kNormWarps) norm_fwd_kernel(const NormFwd
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float c = v[i][j][e] - mean;
-        if (base + norm_col(lane, i, j) + e < lim) sq[0] += c * c;
+        if (base + norm_col<VEC>(lane, i, j, e) < lim) sq[0] += c * c;
       }
-  row_sum<WR, 1>(sq, s_red, warp, lane);
+  row_sum<kNormWarps, WR, 1>(sq, s_red, red, warp, lane);
   const float rstd = valid ? rsqrtf(sq[0] / d + p.eps) : 0.f;
   if (in && warp % WR == 0 && lane == 0) {
     p.mean[row] = mean;
@@ -110,23 +114,22 @@ __global__ void __launch_bounds__(32 * kNormWarps) norm_fwd_kernel(const NormFwd
   const int nb = n_blocks(d);
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    const int c0 = base + 512 * i + 128 * (lane >> 3);
+    const int c0 = base + norm_blk(lane, i), sub = lane & 7;
     const bool live = in && c0 < d;
     if (p.x_codes != nullptr)
       pack_block<VEC>(v[i], c0, d, p.x_codes + at, p.x_scales + (in ? row * nb : 0) + c0 / kBlk, lane & 7, live);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int c = c0 + 4 * ((lane & 7) + 8 * j);
       float g[4], bt[4];
-      load4<float, VEC>(p.gamma, c, lim, g);
-      load4<float, VEC>(p.beta, c, lim, bt);
+      load4<float, VEC>(p.gamma, c0, sub, j, lim, g);
+      load4<float, VEC>(p.beta, c0, sub, j, lim, bt);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[i][j][e] = c + e < lim ? (v[i][j][e] - mean) * rstd * g[e] + bt[e] : 0.f;
+      for (int e = 0; e < 4; ++e) v[i][j][e] = piece_col<VEC>(c0, sub, j, e) < lim ? (v[i][j][e] - mean) * rstd * g[e] + bt[e] : 0.f;
       if constexpr (!std::is_same_v<Y, uint8_t>) {
         Y o[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = from_f32<Y>(v[i][j][e]);
-        if (in) store4<Y, VEC>(static_cast<Y*>(p.y) + at, c, d, o);
+        if (in) store4<Y, VEC>(static_cast<Y*>(p.y) + at, c0, sub, j, d, o);
       }
     }
     if constexpr (std::is_same_v<Y, uint8_t>)
@@ -156,12 +159,15 @@ struct NormBwdParams {
 // a stride; each lane keeps the sums of its own columns, joined over the
 // CTA's row groups at the end and over the CTAs by norm_grad_kernel, always
 // in the same order.
-template <typename DY, typename X, bool X8, int WR, int NI, bool VEC>
-__global__ void __launch_bounds__(32 * kNormWarps, kNormBwdCtas) norm_bwd_kernel(const NormBwdParams p) {
-  constexpr int kGroups = kNormWarps / WR;  // rows in flight per CTA
-  __shared__ float s_red[kNormWarps * 2];
+template <typename DY, typename X, bool X8, int WR, bool VEC>
+__global__ void __launch_bounds__(32 * norm_bwd_warps(WR), norm_bwd_ctas(WR)) norm_bwd_kernel(const NormBwdParams p) {
+  constexpr int NI = 1;
+  constexpr int kWarps = norm_bwd_warps(WR);
+  constexpr int kGroups = kWarps / WR;  // rows in flight per CTA
+  __shared__ float s_red[2][kWarps * 2];
+  int red = 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int base = (warp % WR) * 1024;
+  const int base = (warp % WR) * 512;
   const int d = p.d, nb = n_blocks(d);
   const float inv_d = 1.f / d;
   float acc_w[NI][4][4], acc_b[NI][4][4];
@@ -173,44 +179,61 @@ __global__ void __launch_bounds__(32 * kNormWarps, kNormBwdCtas) norm_bwd_kernel
       for (int e = 0; e < 4; ++e) acc_w[i][j][e] = acc_b[i][j][e] = 0.f;
 
   const long long step = (long long)gridDim.x * kGroups;
+  const int sub = lane & 7;
+  auto valid_at = [&](long long row) { return row < p.rows && (p.mask == nullptr || p.mask[row] != 0); };
+  bool valid = valid_at((long long)blockIdx.x * kGroups + warp / WR);
   // the CTA's row groups run the same number of iterations: row_sum meets at barriers
   for (long long r0 = (long long)blockIdx.x * kGroups; r0 < p.rows; r0 += step) {
     const long long row = r0 + warp / WR;
     const bool in = row < p.rows;
-    const bool valid = in && (p.mask == nullptr || p.mask[row] != 0);
     const int lim = valid ? d : 0;
     const long long at = in ? row * d : 0;
+    // everything that the row needs is on its way before anything waits
     const float mean = valid ? p.mean[row] : 0.f, rstd = valid ? p.rstd[row] : 0.f;
-    float g[NI][4][4], xh[NI][4][4];
+    float g[NI][4][4], xh[NI][4][4], r[NI][4][4];
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        load4<DY, VEC>(static_cast<const DY*>(p.dy) + at, base + norm_col(lane, i, j), lim, g[i][j]);
+        load4<DY, VEC>(static_cast<const DY*>(p.dy) + at, base + norm_blk(lane, i), sub, j, lim, g[i][j]);
     if constexpr (X8) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int c0 = base + norm_col(lane, i, 0);
+        const int c0 = base + norm_blk(lane, i);
         const float s = c0 < lim ? scale_value(p.x_scales[row * nb + c0 / kBlk]) : 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          e4m3x4_value(load_codes4<VEC>(static_cast<const uint8_t*>(p.x) + at, base + norm_col(lane, i, j), lim), s,
-                       xh[i][j]);
+          e4m3x4_value(load_codes4<VEC>(static_cast<const uint8_t*>(p.x) + at, c0, sub, j, lim), s, xh[i][j]);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          load4<X, VEC>(static_cast<const X*>(p.x) + at, base + norm_col(lane, i, j), lim, xh[i][j]);
+          load4<X, VEC>(static_cast<const X*>(p.x) + at, base + norm_blk(lane, i), sub, j, lim, xh[i][j]);
     }
+    if (p.resid != nullptr) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          load4<X, VEC>(static_cast<const X*>(p.resid) + at, base + norm_blk(lane, i), sub, j, lim, r[i][j]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) r[i][j][e] = 0.f;
+    }
+    const bool valid_next = valid_at(row + step);
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float gm[4];
-        load4<float, VEC>(p.gamma, base + norm_col(lane, i, j), d, gm);
+        load4<float, VEC>(p.gamma, base + norm_blk(lane, i), sub, j, d, gm);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float xv = valid ? (xh[i][j][e] - mean) * rstd : 0.f;
@@ -224,27 +247,25 @@ __global__ void __launch_bounds__(32 * kNormWarps, kNormBwdCtas) norm_bwd_kernel
           g[i][j][e] = gv;
         }
       }
-    row_sum<WR, 2>(s, s_red, warp, lane);
+    row_sum<kWarps, WR, 2>(s, s_red, red, warp, lane);
     const float m0 = s[0] * inv_d, m1 = s[1] * inv_d;
     if (in) {
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int c = base + norm_col(lane, i, j);
-          float r[4] = {0.f, 0.f, 0.f, 0.f};
-          if (p.resid != nullptr) load4<X, VEC>(static_cast<const X*>(p.resid) + at, c, lim, r);
           X o[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            o[e] = from_f32<X>(valid ? rstd * (g[i][j][e] - m0 - xh[i][j][e] * m1) + r[e] : 0.f);
-          store4<X, VEC>(static_cast<X*>(p.dx) + at, c, d, o);
+            o[e] = from_f32<X>(valid ? rstd * (g[i][j][e] - m0 - xh[i][j][e] * m1) + r[i][j][e] : 0.f);
+          store4<X, VEC>(static_cast<X*>(p.dx) + at, base + norm_blk(lane, i), sub, j, d, o);
         }
     }
+    valid = valid_next;
   }
 
   // sums over the CTA's row groups, in group order
-  __shared__ float s_acc[kGroups > 1 ? 1024 * NI / 2 : 1];
+  __shared__ float s_acc[kGroups > 1 ? 512 : 1];
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     auto& acc = q == 0 ? acc_w : acc_b;
@@ -262,7 +283,7 @@ __global__ void __launch_bounds__(32 * kNormWarps, kNormBwdCtas) norm_bwd_kernel
 #pragma unroll
               for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s_acc[norm_col(lane, i, j) + e] = acc[i][j][e];
+                for (int e = 0; e < 4; ++e) s_acc[norm_col<VEC>(lane, i, j, e)] = acc[i][j][e];
           __syncthreads();
           if (warp / WR == 0 && warp % WR == half)
 #pragma unroll
@@ -270,7 +291,7 @@ __global__ void __launch_bounds__(32 * kNormWarps, kNormBwdCtas) norm_bwd_kernel
 #pragma unroll
               for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] += s_acc[norm_col(lane, i, j) + e];
+                for (int e = 0; e < 4; ++e) acc[i][j][e] += s_acc[norm_col<VEC>(lane, i, j, e)];
         }
       }
     }
@@ -281,7 +302,7 @@ __global__ void __launch_bounds__(32 * kNormWarps, kNormBwdCtas) norm_bwd_kernel
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int c = base + norm_col(lane, i, j) + e;
+            const int c = base + norm_col<VEC>(lane, i, j, e);
             if (c < d) out[c] = acc[i][j][e];
           }
   }

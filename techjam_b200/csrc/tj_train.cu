@@ -387,7 +387,7 @@ int tj_wgrad8(const void* dy, int dtype, const void* x8_codes, const uint8_t* x8
     tj::wgrad8_join_kernel<<<(unsigned)((total / 4 + 255) / 256), 256, 0, st>>>(p.dw, w.splits, total, dw);
     TJH_CUDA(cudaGetLastError());
   }
-  tj::column_sum_kernel<<<(n + 31) / 32, 256, 0, st>>>(p.db, 4 * w.splits * w.k_tiles, n, db, db, n);
+  tj::column_sum_kernel<<<(n + 7) / 8, 1024, 0, st>>>(p.db, 4 * w.splits * w.k_tiles, n, db, db, n);
   TJH_CUDA(cudaGetLastError());
   return TJ_OK;
 }
