@@ -20,8 +20,9 @@
 //
 // The tensor core truncates when it adds to the accumulator; over 32 steps
 // (1024 of K) that is about 6e-7 of the sum and grows with K.  A 32-bit result
-// therefore starts a new accumulator after each 1024 of K, and the epilogue
-// adds them up in registers, rounded to nearest.
+// and the GELU kind, whose codes would more often fall on the wrong side of a
+// boundary, therefore start a new accumulator after each 1024 of K, and the
+// epilogue adds them up in registers, rounded to nearest.
 #pragma once
 #include "tj_act8.cuh"
 #include "tj_gemm.cuh"
@@ -44,7 +45,7 @@ struct Gemm8Params {
 };
 
 constexpr int kG8BM = 128;
-constexpr int kG8Chunk = 8;  // kG8F32: K blocks per accumulator
+constexpr int kG8Chunk = 8;  // kG8F32, kG8Gelu: K blocks per accumulator
 
 template <int BN, int KIND>
 struct Gemm8Cfg {
@@ -110,6 +111,39 @@ TJ_DEV void bulk_wait_read() {
 }
 TJ_DEV void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
+TJ_DEV void mbar_arrive_cluster_release(uint32_t cluster_addr) {  // one lane of a converged warp
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t.reg .b32 r;\n\t"
+      "elect.sync r|e, 0xffffffff;\n\t"
+      "@e mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n\t}" ::"r"(cluster_addr)
+      : "memory");
+}
+// Plain remote arrive (as mbar_arrive_cluster), by one lane of a converged warp.
+TJ_DEV void mbar_arrive_cluster_elect(uint32_t cluster_addr) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t.reg .b32 r;\n\t"
+      "elect.sync r|e, 0xffffffff;\n\t"
+      "@e mbarrier.arrive.shared::cluster.b64 _, [%0];\n\t}" ::"r"(cluster_addr)
+      : "memory");
+}
+// Bounded wait that also acquires what the other CTA of the pair released.
+TJ_DEV bool mbar_wait_cluster_warp(uint64_t* bar, uint32_t parity, int* err, int site) {
+  auto try_wait = [&] {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+  };
+  if (__all_sync(0xffffffffu, try_wait())) return true;
+  if (!mbar_wait_warp(bar, parity, err, site)) return false;
+  return __all_sync(0xffffffffu, try_wait());  // complete: returns at once, with the acquire
+}
+
 // Four bytes of a scale row from block b0 on (byte loads: rows start anywhere); past the end 2^0.
 TJ_DEV uint32_t scale_word(const uint8_t* row, int b0, int blocks) {
   uint32_t w = 0;
@@ -138,6 +172,72 @@ TJ_DEV uint32_t pack_bf162(float a, float b) {
 // 16-byte piece j of this lane's 128-byte row in a 32-row staging buffer (the
 // 128-byte TMA swizzle; conflict-free for one piece per lane).
 TJ_DEV uint8_t* staged(uint8_t* buf, int lane, int j) { return buf + lane * 128 + ((j ^ (lane & 7)) << 4); }
+
+// GELU epilogue of one row's block of 128: h in 32 bits -> staged codes of
+// g = gelu(h) and of h, and their scale bytes (rows that are not valid: zeros).
+// gelu grows with h > 0 and its dip for h < 0 is 0.17 deep, which gelu(0.3)
+// exceeds: above that the largest |g| is gelu of the largest h, and only a
+// warp with a smaller one looks at every g.  Called by whole warps.
+TJ_DEV void gelu_pack_row(float (&h)[128], bool valid, uint8_t* bufg, uint8_t* bufh, int lane, uint32_t& gbyte,
+                          uint32_t& hbyte) {
+  float hmax = 0.f, hpos = 0.f;
+  auto maxima = [&] {
+    float m[4] = {0.f, 0.f, 0.f, 0.f}, q[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 128; i += 8)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        m[k] = max3f(m[k], fabsf(h[i + 2 * k]), fabsf(h[i + 2 * k + 1]));
+        q[k] = max3f(q[k], h[i + 2 * k], h[i + 2 * k + 1]);
+      }
+    hmax = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+    hpos = fmaxf(fmaxf(q[0], q[1]), fmaxf(q[2], q[3]));
+  };
+  maxima();
+  if (__any_sync(0xffffffffu, hmax > 3.402823466e38f)) {  // infinities become NaN, which the maxima drop
+#pragma unroll
+    for (int i = 0; i < 128; ++i)
+      if (fabsf(h[i]) > 3.402823466e38f) h[i] = __int_as_float(0x7fffffff);
+    maxima();
+  }
+  float gmax = gelu_erf_x2(hpos, 0.f).x;
+  if (__any_sync(0xffffffffu, hpos < 0.3f)) {
+#pragma unroll
+    for (int i = 0; i < 128; i += 2) {
+      const float2 g = gelu_erf_x2(h[i], h[i + 1]);
+      gmax = max3f(gmax, fabsf(g.x), fabsf(g.y));
+    }
+  }
+  gbyte = valid ? scale_byte(gmax) : 127u;
+  hbyte = valid ? scale_byte(hmax) : 127u;
+  const float ginv = scale_inv(gbyte), hinv = scale_inv(hbyte);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    uint32_t gw[4], hw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float* v = h + 16 * j + 4 * i;
+      const float2 g0 = gelu_erf_x2(v[0], v[1]), g1 = gelu_erf_x2(v[2], v[3]);
+      gw[i] = e4m3x2<false>(g0.x, g0.y, ginv) | (e4m3x2<false>(g1.x, g1.y, ginv) << 16);
+      hw[i] = e4m3x2<false>(v[0], v[1], hinv) | (e4m3x2<false>(v[2], v[3], hinv) << 16);
+    }
+    *reinterpret_cast<uint4*>(staged(bufg, lane, j)) =
+        valid ? make_uint4(gw[0], gw[1], gw[2], gw[3]) : make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(staged(bufh, lane, j)) =
+        valid ? make_uint4(hw[0], hw[1], hw[2], hw[3]) : make_uint4(0, 0, 0, 0);
+  }
+}
+
+// Adds the bias of columns col0.. (zeros past n) to 32 values.
+TJ_DEV void add_bias32(float* v, const float* bias, int col0, int n) {
+  if (bias == nullptr) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (col0 + 4 * j < n) {
+      const float4 b = __ldg(reinterpret_cast<const float4*>(bias + col0) + j);
+      v[4 * j] += b.x; v[4 * j + 1] += b.y; v[4 * j + 2] += b.z; v[4 * j + 3] += b.w;
+    }
+}
 
 template <int BN, int KIND>
 __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
@@ -182,7 +282,7 @@ __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
   const int m_tiles = (p.M + kG8BM - 1) / kG8BM;
   const long long total = (long long)m_tiles * n_tiles;
   const int kblocks = p.kblocks;
-  constexpr int kChunk = KIND == kG8F32 ? kG8Chunk : 1 << 30;  // K blocks per accumulator
+  constexpr int kChunk = KIND == kG8F32 || KIND == kG8Gelu ? kG8Chunk : 1 << 30;  // K blocks per accumulator
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
@@ -427,91 +527,36 @@ __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
           ++used;
         }
       } else {
-        // GELU: this warp's 128 columns are one block of g = gelu(h) and of
-        // h = acc + bias, and a thread holds a whole row of it.  First pass
-        // over the accumulator: the two maxima.  Second: the codes.
-        float hmax = 0.f, hpos = 0.f, gmax = 0.f;
+        // GELU: this warp's 128 columns are one block of g and of h, and a
+        // thread holds a whole row of it
         const bool store = row0 < p.M && col0 < p.N;
+        uint32_t gbyte = 127u, hbyte = 127u;
         uint8_t* bufg = bufs + (used % Cfg::kBufs) * 4096;
         uint8_t* bufh = bufs + ((used + 1) % Cfg::kBufs) * 4096;
-        auto load_h = [&](int c, float (&h)[32]) {
-          uint32_t r[32];
-          tmem_ld32(taddr + abuf * BN + 32 * c, r);
-          tmem_ld_wait();
+        float h[128];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float4 bb = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (p.bias != nullptr && col0 + 32 * c + 4 * j < p.N)
-              bb = __ldg(reinterpret_cast<const float4*>(p.bias + col0 + 32 * c) + j);
-            h[4 * j] = __uint_as_float(r[4 * j]) + bb.x;
-            h[4 * j + 1] = __uint_as_float(r[4 * j + 1]) + bb.y;
-            h[4 * j + 2] = __uint_as_float(r[4 * j + 2]) + bb.z;
-            h[4 * j + 3] = __uint_as_float(r[4 * j + 3]) + bb.w;
-          }
-        };
-        uint32_t gbyte = 127u, hbyte = 127u;
+        for (int i = 0; i < 128; ++i) h[i] = 0.f;
         if (live) {
-          if (!wait_acc()) break;
-          for (int c = 0; c < 4; ++c) {
-            float h[32];
-            load_h(c, h);
+          for (int kb = 0; kb < kblocks; kb += kChunk) {
+            if (!wait_acc()) break;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float a = finite_abs(h[i]);
-              hmax = fmaxf(hmax, a);
-              if (h[i] > 0.f) hpos = fmaxf(hpos, a);
-            }
-          }
-          // gelu grows with h > 0 and its dip for h < 0 is 0.17 deep, which
-          // gelu(0.3) exceeds: above that the largest |g| is gelu(hpos)
-          gmax = gelu_erf_x2(hpos, 0.f).x;
-          if (__any_sync(0xffffffffu, hpos < 0.3f)) {
             for (int c = 0; c < 4; ++c) {
-              float h[32];
-              load_h(c, h);
+              uint32_t r[32];
+              tmem_ld32(taddr + abuf * BN + 32 * c, r);
+              tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; i += 2) {
-                const float2 g = gelu_erf_x2(h[i], h[i + 1]);
-                gmax = fmaxf(gmax, fmaxf(finite_abs(g.x), finite_abs(g.y)));
-              }
+              for (int i = 0; i < 32; ++i) h[32 * c + i] += __uint_as_float(r[i]);
             }
+            free_acc();
           }
-          gbyte = valid ? scale_byte(gmax) : 127u;
-          hbyte = valid ? scale_byte(hmax) : 127u;
+          if (!ok) break;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) add_bias32(h + 32 * c, p.bias, col0 + 32 * c, p.N);
         }
         if (store) {
           if (lane == 0) bulk_wait_read<2>();
           __syncwarp();
-        }
-        const float ginv = scale_inv(gbyte), hinv = scale_inv(hbyte);
-        for (int c = 0; c < 4; ++c) {
-          uint32_t gw[8], hw[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) gw[i] = hw[i] = 0u;
-          if (live) {
-            float h[32];
-            load_h(c, h);
-            if (c == 3) free_acc();
-            if (valid) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float2 g0 = gelu_erf_x2(h[4 * i], h[4 * i + 1]), g1 = gelu_erf_x2(h[4 * i + 2], h[4 * i + 3]);
-                gw[i] = e4m3x2<true>(g0.x, g0.y, ginv) | (e4m3x2<true>(g1.x, g1.y, ginv) << 16);
-                hw[i] = e4m3x2<true>(h[4 * i], h[4 * i + 1], hinv) | (e4m3x2<true>(h[4 * i + 2], h[4 * i + 3], hinv) << 16);
-              }
-            }
-          }
-          if (store) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              *reinterpret_cast<uint4*>(staged(bufg, lane, 2 * c + j)) =
-                  make_uint4(gw[4 * j], gw[4 * j + 1], gw[4 * j + 2], gw[4 * j + 3]);
-              *reinterpret_cast<uint4*>(staged(bufh, lane, 2 * c + j)) =
-                  make_uint4(hw[4 * j], hw[4 * j + 1], hw[4 * j + 2], hw[4 * j + 3]);
-            }
-          }
-        }
-        if (store) {
+          gelu_pack_row(h, valid, bufg, bufh, lane, gbyte, hbyte);
           fence_async_smem();
           __syncwarp();
           if (lane == 0) {
@@ -535,6 +580,347 @@ __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
   __syncthreads();
   tc_fence_after();
   if (warp == 2) tmem_dealloc(tmem_base, Cfg::kTmemCols);
+}
+
+// ------------------------------------------------------------------ CTA pairs
+// A pair computes 256 x 256 tiles with cta_group::2: each CTA stages 128 rows
+// of A and 128 of the 256 W rows, 32 KB for 512 cycles of MMA (a 128 x 128
+// tile of one CTA needs 32 KB for 256, twice what an SM gets from L2).
+//
+// TMEM holds two 256-column accumulators and the scales only because the
+// accumulators overlap by 32 columns: buffer 0 has columns 0-255, buffer 1
+// columns 224-479.  The epilogue of a tile therefore reads the shared columns
+// first and announces them (`shared_free`), and the next tile's MMAs wait for
+// that besides their buffer.  Meanwhile the operand ring fills, so that the
+// loads, which bound the kernel, do not pause.
+template <int KIND>
+struct Gemm8PairCfg {
+  static constexpr int kBN = 256;
+  static constexpr int kStageBytes = 2 * 128 * 128;
+  static constexpr int kBufs = 2;
+  static constexpr int kStagingBytes = 8 * kBufs * 4096;
+  static constexpr int kStages = 5;
+  static constexpr int kAcc1 = 224;   // first column of buffer 1
+  static constexpr int kSfCol0 = 480;
+  static constexpr int kSfSlots = 2;
+  static constexpr int kSfCols = 12;  // 4 for A's 128 rows, 8 for W's 256
+  static constexpr int kThreads = 512;
+  static constexpr int kRegLaunch = 128;  // kG8Gelu: warpgroups with 56 + 56 + 2 * 200
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kStagingBytes + 512;
+  static_assert(kSmemBytes <= 232448, "shared memory");
+};
+
+TJ_DEV void umma_mx8_pair_elect(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
+                                uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred e, p;\n\t.reg .b32 r;\n\t"
+      "elect.sync r|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+          d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(512, 1)
+    gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
+                      const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ CUtensorMap tmAux,
+                      const Gemm8Params p) {
+  static_assert(KIND == kG8F16 || KIND == kG8BF16 || KIND == kG8Gelu, "kind");
+  using Cfg = Gemm8PairCfg<KIND>;
+  constexpr int S = Cfg::kStages, SF = Cfg::kSfSlots;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* staging = smem + S * Cfg::kStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + Cfg::kStagingBytes);  // [S] (even CTA's copy)
+  uint64_t* empty = full + S;             // [S]
+  uint64_t* acc_full = empty + S;         // [2]
+  uint64_t* acc_empty = acc_full + 2;     // [2] (even CTA's copy)
+  uint64_t* shared_free = acc_empty + 2;  // the shared columns are read (even CTA's copy)
+  uint64_t* sf_full = shared_free + 1;    // [SF] (even CTA's copy)
+  uint64_t* sf_empty = sf_full + SF;      // [SF]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sf_empty + SF);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(acc_full + i, 1); mbar_init(acc_empty + i, 16); }
+    mbar_init(shared_free, 8);
+    for (int i = 0; i < SF; ++i) { mbar_init(sf_full + i, 8); mbar_init(sf_empty + i, 1); }
+    fence_mbar_init();
+  }
+  if (warp == 2) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int n_tiles = (p.N + 255) / 256;
+  const int m_tiles = (p.M + 255) / 256;
+  const long long total = (long long)m_tiles * n_tiles;
+  const int kblocks = p.kblocks;
+  constexpr int kChunk = KIND == kG8Gelu ? kG8Chunk : 1 << 30;
+  // both CTAs take or leave a tile together
+  auto pair_has_rows = [&](int mt) {
+    return tile_has_rows(p.mask, mt * 256, p.M, lane) || tile_has_rows(p.mask, mt * 256 + 128, p.M, lane);
+  };
+
+  if (warp < 4) {
+    if constexpr (KIND == kG8Gelu) reg_dealloc<56>();
+    if (warp == 0) {
+      // ---------------------------------------------------------- TMA producer
+      if (lane == 0) { tma_prefetch_desc(&tmA); tma_prefetch_desc(&tmW); }
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (long long t = pair; t < total && ok; t += n_pairs) {
+        const int mt = (int)(t / n_tiles), nt = (int)(t % n_tiles);
+        if (!pair_has_rows(mt)) continue;
+        if (lane == 0) {
+          for (int kb = 0; kb < kblocks; ++kb) {
+            if (!mbar_wait(empty + stage, phase ^ 1u, p.err, kErrGemm8Producer)) { ok = false; break; }
+            uint8_t* sa = smem + stage * Cfg::kStageBytes;
+            const uint32_t lb = pair_leader_bar(full + stage);
+            if (rank == 0) mbar_expect_tx(full + stage, 2 * Cfg::kStageBytes);
+            tma_load_2d_pair(sa, &tmA, lb, kb * 128, mt * 256 + (int)rank * 128);
+            tma_load_2d_pair(sa + 16384, &tmW, lb, kb * 128, nt * 256 + (int)rank * 128);
+            if (++stage == S) { stage = 0; phase ^= 1u; }
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+      }
+      // after an expired wait: give the last loads time to land
+      if (!ok && lane == 0) {
+        const uint64_t t = global_ns();
+        while (global_ns() - t < 100000) {
+        }
+      }
+    } else if (warp == 1 && rank == 0) {
+      // ---------------------------------------------------------- MMA issuer
+      int stage = 0, abuf = 0, slot = 0;
+      uint32_t phase = 0, aphase = 0, sphase = 0, shphase = 0;
+      bool ok = true, any = false;
+      for (long long t = pair; t < total && ok; t += n_pairs) {
+        if (!pair_has_rows((int)(t / n_tiles))) continue;
+        for (int kb = 0; kb < kblocks; ++kb) {
+          const bool first = kb % kChunk == 0;
+          if (first) {
+            if (!mbar_wait_warp(acc_empty + abuf, aphase ^ 1u, p.err, kErrGemm8Mma)) { ok = false; break; }
+            if (any) {  // the accumulator before this one has given up the shared columns
+              if (!mbar_wait_warp(shared_free, shphase, p.err, kErrGemm8Mma)) { ok = false; break; }
+              shphase ^= 1u;
+            }
+            any = true;
+          }
+          if ((kb & 3) == 0) {
+            if (!mbar_wait_cluster_warp(sf_full + slot, sphase, p.err, kErrGemm8Mma)) { ok = false; break; }
+          }
+          if (!mbar_wait_warp(full + stage, phase, p.err, kErrGemm8Mma)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + stage * Cfg::kStageBytes);
+          const uint32_t sfa = tmem_base + Cfg::kSfCol0 + slot * Cfg::kSfCols;
+          const uint32_t idesc = idesc_mx8(256, 256) | idesc_mx8_ids(kb & 3);
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            umma_mx8_pair_elect(tmem_base + abuf * Cfg::kAcc1, smem_desc(sa + ks * 32, 16, 1024, 128),
+                                smem_desc(sa + 16384 + ks * 32, 16, 1024, 128), idesc, sfa, sfa + 4,
+                                !(first && ks == 0));
+          umma_commit_pair_both_elect(empty + stage);
+          if (++stage == S) { stage = 0; phase ^= 1u; }
+          if ((kb & 3) == 3 || kb + 1 == kblocks) {
+            umma_commit_pair_both_elect(sf_empty + slot);
+            if (++slot == SF) { slot = 0; sphase ^= 1u; }
+          }
+          if (kb % kChunk == kChunk - 1 || kb + 1 == kblocks) {
+            umma_commit_pair_both_elect(acc_full + abuf);
+            if (++abuf == 2) { abuf = 0; aphase ^= 1u; }
+          }
+        }
+      }
+    }
+  } else if (warp < 8) {
+    // ------------------------------------------------------------ scales -> TMEM
+    if constexpr (KIND == kG8Gelu) reg_dealloc<56>();
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t sf_full0 = map_to_rank(sf_full, 0);
+    int slot = 0;
+    uint32_t sphase = 0;
+    bool ok = true;
+    for (long long t = pair; t < total && ok; t += n_pairs) {
+      const int mt = (int)(t / n_tiles), nt = (int)(t % n_tiles);
+      if (!pair_has_rows(mt)) continue;
+      const uint8_t* wrow0 = p.w_scales + (long long)(2 * nt) * kblocks;
+      const bool two = nt * 256 + 128 < p.N;
+      for (int kb = 0; kb < kblocks; kb += 4) {
+        uint32_t a[4], b[8];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int row = mt * 256 + (int)rank * 128 + 32 * c + lane;
+          a[c] = row < p.M ? scale_word(p.a_scales + (long long)row * kblocks, kb, kblocks) : 0x7f7f7f7fu;
+        }
+        b[0] = scale_word(wrow0, kb, kblocks);
+        b[4] = two ? scale_word(wrow0 + kblocks, kb, kblocks) : 0x7f7f7f7fu;
+#pragma unroll
+        for (int c = 1; c < 4; ++c) { b[c] = b[0]; b[4 + c] = b[4]; }
+        if (!mbar_wait_warp(sf_empty + slot, sphase ^ 1u, p.err, kErrGemm8Scales)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t at = tmem_base + lanes + Cfg::kSfCol0 + slot * Cfg::kSfCols;
+        tmem_st_words<4>(at, a);
+        tmem_st_words<8>(at + 4, b);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive_cluster_release(sf_full0 + (uint32_t)(slot * sizeof(uint64_t)));
+        if (++slot == SF) { slot = 0; sphase ^= 1u; }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    if constexpr (KIND == kG8Gelu) reg_alloc<200>();
+    const int ew = warp - 8, quarter = warp & 3, half = ew >> 2;
+    uint8_t* bufs = staging + ew * Cfg::kBufs * 4096;
+    const uint32_t acc_empty0 = map_to_rank(acc_empty, 0), shared_free0 = map_to_rank(shared_free, 0);
+    uint32_t used = 0;  // staging buffers used so far
+    int abuf = 0;
+    uint32_t aphase = 0;
+    bool ok = true;
+    for (long long t = pair; t < total && ok; t += n_pairs) {
+      const int mt = (int)(t / n_tiles), nt = (int)(t % n_tiles);
+      const bool live = pair_has_rows(mt);
+      const int row0 = mt * 256 + (int)rank * 128 + quarter * 32;
+      const int col0 = nt * 256 + half * 128;
+      const int row = row0 + lane;
+      const bool valid = row < p.M && (p.mask == nullptr || __ldg(p.mask + row) != 0);
+      auto wait_acc = [&] {
+        ok = mbar_wait_warp(acc_full + abuf, aphase, p.err, kErrGemm8Epilogue);
+        tc_fence_after();
+        return ok;
+      };
+      auto acc_addr = [&] { return tmem_base + ((uint32_t)(quarter * 32) << 16) + abuf * Cfg::kAcc1 + half * 128; };
+      auto free_shared = [&] {
+        tc_fence_before();
+        mbar_arrive_cluster_elect(shared_free0);
+      };
+      auto free_acc = [&] {
+        tc_fence_before();
+        mbar_arrive_cluster_elect(acc_empty0 + (uint32_t)(abuf * sizeof(uint64_t)));
+        if (++abuf == 2) { abuf = 0; aphase ^= 1u; }
+      };
+      if constexpr (KIND == kG8Gelu) {
+        float h[128];
+#pragma unroll
+        for (int i = 0; i < 128; ++i) h[i] = 0.f;
+        if (live) {
+          for (int kb = 0; kb < kblocks; kb += kChunk) {
+            if (!wait_acc()) break;
+            // buffer 0 shares its last 32 columns, buffer 1 its first: both
+            // are this warp's piece 3 or 0, if they are in its half at all
+            const uint32_t taddr = acc_addr();
+            const bool mine = half == (abuf ^ 1);
+            if (mine) {
+              uint32_t r[32];
+              if (abuf == 0) {
+                tmem_ld32(taddr + 96, r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) h[96 + i] += __uint_as_float(r[i]);
+              } else {
+                tmem_ld32(taddr, r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) h[i] += __uint_as_float(r[i]);
+              }
+              free_shared();
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              if (mine && c == (abuf == 0 ? 3 : 0)) continue;  // warp-uniform
+              uint32_t r[32];
+              tmem_ld32(taddr + 32 * c, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) h[32 * c + i] += __uint_as_float(r[i]);
+            }
+            free_acc();
+          }
+          if (!ok) break;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) add_bias32(h + 32 * c, p.bias, col0 + 32 * c, p.N);
+        }
+        if (row0 < p.M && col0 < p.N) {
+          uint32_t gbyte, hbyte;
+          if (lane == 0) bulk_wait_read<0>();
+          __syncwarp();
+          gelu_pack_row(h, valid, bufs, bufs + 4096, lane, gbyte, hbyte);
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&tmOut, bufs, col0, row0);
+            tma_store_2d(&tmAux, bufs + 4096, col0, row0);
+            bulk_commit();
+          }
+          if (row < p.M) {
+            const long long s = (long long)row * n_blocks(p.N) + col0 / kBlk;
+            p.g_scales[s] = (uint8_t)gbyte;
+            p.h_scales[s] = (uint8_t)hbyte;
+          }
+        }
+      } else {
+        if (live && !wait_acc()) break;
+        const int cur = abuf;
+        const uint32_t taddr = acc_addr();
+        const bool mine = half == (cur ^ 1);
+        // two 64-column pieces, the one with the shared columns first
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int piece = cur == 0 && half == 1 ? 1 - q : q;
+          const int col = col0 + 64 * piece;
+          uint32_t r[2][32];
+          if (live) {
+            tmem_ld32(taddr + 64 * piece, r[0]);
+            tmem_ld32(taddr + 64 * piece + 32, r[1]);
+            tmem_ld_wait();
+            if (q == 0 && mine) free_shared();
+            if (q == 1) free_acc();
+          }
+          if (row0 >= p.M || col >= p.N) continue;
+          uint32_t w[32];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float* v = reinterpret_cast<float*>(r[c]);
+            if (live) add_bias32(v, p.bias, col + 32 * c, p.N);
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              w[16 * c + j] = KIND == kG8F16 ? pack_half2(v[2 * j], v[2 * j + 1]) : pack_bf162(v[2 * j], v[2 * j + 1]);
+          }
+          uint8_t* buf = bufs + (used++ & 1) * 4096;
+          if (lane == 0) bulk_wait_read<1>();  // the store of this buffer is the one before last
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4*>(staged(buf, lane, j)) =
+                valid ? make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]) : make_uint4(0, 0, 0, 0);
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&tmOut, buf, col, row0);
+            bulk_commit();
+          }
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_all();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  if (warp == 2) tmem_dealloc_pair(tmem_base, 512);
 }
 
 }  // namespace tj

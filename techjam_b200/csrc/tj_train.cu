@@ -122,6 +122,66 @@ int launch_gemm8(const Gemm8Args& g, const tj::Gemm8Params& p, int dev, int sms,
   return TJ_OK;
 }
 
+// CTA pairs that run at once, and the kernel's attributes, once per device.
+template <typename K>
+int cluster_pairs(K kern, cudaLaunchConfig_t cfg, int regs, int dev, int (&max_pairs)[64], std::mutex& mu, int* pairs) {
+  std::lock_guard<std::mutex> lock(mu);
+  if (dev < 0 || dev >= 64) return fail(TJ_ERR_NO_DEVICE, "device index %d out of range", dev);
+  if (max_pairs[dev] == 0) {
+    // The warpgroups' register budgets add up to what the launch gives; with
+    // any other count an increase would wait for registers that nobody frees,
+    // so refuse to launch.
+    cudaFuncAttributes fa;
+    TJH_CUDA(cudaFuncGetAttributes(&fa, kern));
+    if (regs != 0 && fa.numRegs != regs)
+      return fail(TJ_ERR_UNSUPPORTED, "kernel built with %d registers per thread, needs %d", fa.numRegs, regs);
+    TJH_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes));
+    cfg.gridDim = dim3(2);
+    int n = 0;
+    TJH_CUDA(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+    max_pairs[dev] = n > 0 ? n : 1;
+  }
+  *pairs = max_pairs[dev];
+  return TJ_OK;
+}
+struct PairLaunch {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  PairLaunch(int threads, int smem, cudaStream_t st) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+};
+
+template <int KIND>
+int launch_gemm8_pair(const Gemm8Args& g, const tj::Gemm8Params& p, int dev, cudaStream_t st) {
+  using Cfg = tj::Gemm8PairCfg<KIND>;
+  auto kern = tj::gemm8_pair_kernel<KIND>;
+  static std::mutex mu;
+  static int max_pairs[64] = {};
+  PairLaunch l(Cfg::kThreads, Cfg::kSmemBytes, st);
+  int pairs = 0;
+  TJH_CHECK(cluster_pairs(kern, l.cfg, KIND == tj::kG8Gelu ? Cfg::kRegLaunch : 0, dev, max_pairs, mu, &pairs));
+  CUtensorMap ta, tw, to, tx;
+  TJH_CHECK(tj_host::make_map(&ta, g.a, 1, p.M, p.K, 128, 128));
+  TJH_CHECK(tj_host::make_map(&tw, g.w, 1, p.N, p.K, 128, 128));
+  constexpr int elt = KIND == tj::kG8Gelu ? 1 : 2;
+  TJH_CHECK(tj_host::make_map(&to, g.out, elt, p.M, p.N, 32, 128 / elt));
+  tx = to;
+  if (KIND == tj::kG8Gelu) TJH_CHECK(tj_host::make_map(&tx, g.aux_out, 1, p.M, p.N, 32, 128));
+  const long long tiles = (long long)((p.M + 255) / 256) * ((p.N + 255) / 256);
+  l.cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(tiles, pairs));
+  TJH_CUDA(cudaLaunchKernelEx(&l.cfg, kern, ta, tw, to, tx, p));
+  return TJ_OK;
+}
+
 int gemm8_params(tj::Gemm8Params* p, const void* a, const uint8_t* as, const void* w, const uint8_t* ws,
                  const float* bias, int m, int n, int k, const uint8_t* mask, int* err) {
   if (m < 0 || n <= 0 || k <= 0) return fail(TJ_ERR_INVALID, "product of [%d, %d] and [%d, %d]", m, k, n, k);
@@ -136,6 +196,11 @@ int gemm8_params(tj::Gemm8Params* p, const void* a, const uint8_t* as, const voi
 
 template <int KIND>
 int gemm8_kind(const Gemm8Args& g, const tj::Gemm8Params& p, int dev, int sms, cudaStream_t st) {
+  if constexpr (KIND != tj::kG8F32) {
+    // 256 x 256 tiles of CTA pairs once they fill the GPU
+    const long long pair_tiles = (long long)((p.M + 255) / 256) * ((p.N + 255) / 256);
+    if (2 * pair_tiles >= sms) return launch_gemm8_pair<KIND>(g, p, dev, st);
+  }
   if constexpr (KIND != tj::kG8Gelu) {
     // few tiles: half as wide, so that twice as many SMs share the weight's bytes
     const long long tiles = (long long)((p.M + 127) / 128) * ((p.N + 127) / 128);
@@ -172,43 +237,15 @@ int launch_wgrad8(const void* dy, const void* x, const tj::Wgrad8Params& p, int 
   auto kern = tj::wgrad8_kernel<T>;
   static std::mutex mu;
   static int max_pairs[64] = {};
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(tj::kWgThreads);
-  cfg.dynamicSmemBytes = tj::kWgSmemBytes;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  PairLaunch l(tj::kWgThreads, tj::kWgSmemBytes, st);
   int pairs = 0;
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    if (dev < 0 || dev >= 64) return fail(TJ_ERR_NO_DEVICE, "device index %d out of range", dev);
-    if (max_pairs[dev] == 0) {
-      // The warpgroups' register budgets (48 + 112 + 2 * 176) add up to the
-      // launch's 4 * 128; with any other count an increase would wait for
-      // registers that nobody frees, so refuse to launch.
-      cudaFuncAttributes fa;
-      TJH_CUDA(cudaFuncGetAttributes(&fa, kern));
-      if (fa.numRegs != tj::kWgRegLaunch)
-        return fail(TJ_ERR_UNSUPPORTED, "weight-gradient kernel built with %d registers per thread, needs %d", fa.numRegs, tj::kWgRegLaunch);
-      TJH_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, tj::kWgSmemBytes));
-      cfg.gridDim = dim3(2);
-      int n = 0;
-      TJH_CUDA(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
-      max_pairs[dev] = n > 0 ? n : 1;
-    }
-    pairs = max_pairs[dev];
-  }
+  TJH_CHECK(cluster_pairs(kern, l.cfg, tj::kWgRegLaunch, dev, max_pairs, mu, &pairs));
   CUtensorMap ty, tx;
   TJH_CHECK(tj_host::make_map(&ty, dy, 2, p.T, p.N, tj::kWgTok, 64));
   TJH_CHECK(tj_host::make_map(&tx, x, 2, p.T, p.K, tj::kWgTok, 64));
   const long long items = (long long)((p.N + 255) / 256) * ((p.K + 255) / 256) * p.splits;
-  cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(items, pairs));
-  TJH_CUDA(cudaLaunchKernelEx(&cfg, kern, ty, tx, p));
+  l.cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(items, pairs));
+  TJH_CUDA(cudaLaunchKernelEx(&l.cfg, kern, ty, tx, p));
   return TJ_OK;
 }
 

@@ -44,7 +44,7 @@ constexpr int kWgChunk = 8;    // stages per accumulator
 constexpr int kWgStages = 7;
 constexpr int kWgStageBytes = 2 * 64 * 128 * 2;  // 128 columns of dY and of X, 64 tokens, 16 bits
 constexpr int kWgThreads = 512;
-constexpr int kWgRegLaunch = 128;
+constexpr int kWgRegLaunch = 128;  // warpgroups with 48 + 112 + 2 * 176
 constexpr int kWgSmemBytes = 1024 + kWgStages * kWgStageBytes + 512;
 
 struct Wgrad8Params {
@@ -124,39 +124,6 @@ __global__ void __launch_bounds__(256) wgrad8_join_kernel(const float* __restric
     a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
   }
   *reinterpret_cast<float4*>(out + i) = a;
-}
-
-TJ_DEV void mbar_arrive_cluster_release(uint32_t cluster_addr) {  // one lane of a converged warp
-  asm volatile(
-      "{\n\t.reg .pred e;\n\t.reg .b32 r;\n\t"
-      "elect.sync r|e, 0xffffffff;\n\t"
-      "@e mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n\t}" ::"r"(cluster_addr)
-      : "memory");
-}
-// Plain remote arrive (as mbar_arrive_cluster), by one lane of a converged warp.
-TJ_DEV void mbar_arrive_cluster_elect(uint32_t cluster_addr) {
-  asm volatile(
-      "{\n\t.reg .pred e;\n\t.reg .b32 r;\n\t"
-      "elect.sync r|e, 0xffffffff;\n\t"
-      "@e mbarrier.arrive.shared::cluster.b64 _, [%0];\n\t}" ::"r"(cluster_addr)
-      : "memory");
-}
-// Bounded wait that also acquires what the other CTA of the pair released.
-TJ_DEV bool mbar_wait_cluster_warp(uint64_t* bar, uint32_t parity, int* err, int site) {
-  auto try_wait = [&] {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-  };
-  if (__all_sync(0xffffffffu, try_wait())) return true;
-  if (!mbar_wait_warp(bar, parity, err, site)) return false;
-  return __all_sync(0xffffffffu, try_wait());  // complete: returns at once, with the acquire
 }
 
 template <typename T>

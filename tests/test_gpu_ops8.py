@@ -349,7 +349,9 @@ def product_tolerance(av, wv, k, out, acc, steps):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 8, 16), (1, 4096, 1024), (128, 128, 128), (129, 136, 144), (300, 264, 1040),
-                                   (777, 1000, 528), (257, 2048, 640), (64, 64, 4112), (2000, 1024, 256)])
+                                   (777, 1000, 528), (257, 2048, 640), (64, 64, 4112), (2000, 1024, 256),
+                                   # enough 256 x 256 tiles for CTA pairs, ragged in each direction
+                                   (2500, 2056, 272), (2304, 2304, 1168), (19000, 200, 32)])
 @pytest.mark.parametrize("out", F)
 def test_product(m, n, k, out):
     a, w = product_inputs(m, n, k, m + n + k)
@@ -372,9 +374,10 @@ def test_product(m, n, k, out):
     assert ops.device_error() == 0
 
 
+@pytest.mark.parametrize("n_tok,n", [(130, 256), (1100, 1024)])
 @pytest.mark.parametrize("out", F)
-def test_product_masked_rows(out):
-    b, n_tok, n, k = 5, 130, 256, 256
+def test_product_masked_rows(out, n_tok, n):
+    b, k = 5, 256
     m = padding(b, n_tok, 4, hole=True)
     m[2] = False  # whole tiles without a valid row
     m[3] = False
@@ -396,7 +399,8 @@ def test_product_masked_rows(out):
 
 
 @pytest.mark.parametrize("m,n,k,scale", [(1, 16, 16, 1.0), (129, 144, 144, 1.0), (300, 2048, 512, 0.05),
-                                         (1000, 512, 256, 4.0), (257, 1024, 1024, 1.0)])
+                                         (1000, 512, 256, 4.0), (257, 1024, 1024, 1.0),
+                                         (2500, 2064, 272, 1.0), (130, 256, 1168, 0.5), (2304, 2304, 1168, 0.2)])
 def test_ffn_in(m, n, k, scale):
     """h and gelu(h) in 8 bits.  A value may land on the code next to the
     exact one's (the accumulator's error can carry it over a boundary), so the
