@@ -38,6 +38,7 @@ struct Gemm8Params {
   const uint8_t* w_scales;  // [ceil(N / 128), kblocks]
   const float* bias;        // [N] or null
   const uint8_t* mask;      // [M] or null: rows with 0 leave zeros
+  int a_words, w_words;     // scale rows may be read as 32-bit words
   int has_resid;            // kG8F32: resid through its tensor map
   uint8_t* g_scales;        // kG8Gelu: [M, ceil(N / 128)]
   uint8_t* h_scales;
@@ -144,8 +145,10 @@ TJ_DEV bool mbar_wait_cluster_warp(uint64_t* bar, uint32_t parity, int* err, int
   return __all_sync(0xffffffffu, try_wait());  // complete: returns at once, with the acquire
 }
 
-// Four bytes of a scale row from block b0 on (byte loads: rows start anywhere); past the end 2^0.
-TJ_DEV uint32_t scale_word(const uint8_t* row, int b0, int blocks) {
+// Four bytes of a scale row from block b0 on; past the end 2^0.  words: the
+// rows start at multiples of 4 and are multiples of 4 long.
+TJ_DEV uint32_t scale_word(const uint8_t* row, int b0, int blocks, bool words) {
+  if (words) return __ldg(reinterpret_cast<const uint32_t*>(row + b0));
   uint32_t w = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) w |= (uint32_t)(b0 + i < blocks ? __ldg(row + b0 + i) : 127) << (8 * i);
@@ -354,16 +357,19 @@ __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
       const int mt = (int)(t / n_tiles), nt = (int)(t % n_tiles);
       if (!tile_has_rows(p.mask, mt * kG8BM, p.M, lane)) continue;
       const uint8_t* wrow = p.w_scales + (long long)(nt * BN / kBlk) * kblocks;
-      for (int kb = 0; kb < kblocks; kb += 4) {
-        uint32_t a[4], b[BN / 32];
+      uint32_t a[4], b[BN / 32];
+      auto fetch = [&](int kb) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const int row = mt * kG8BM + 32 * c + lane;
-          a[c] = row < p.M ? scale_word(p.a_scales + (long long)row * kblocks, kb, kblocks) : 0x7f7f7f7fu;
+          a[c] = row < p.M ? scale_word(p.a_scales + (long long)row * kblocks, kb, kblocks, p.a_words) : 0x7f7f7f7fu;
         }
-        b[0] = scale_word(wrow, kb, kblocks);
+        b[0] = scale_word(wrow, kb, kblocks, p.w_words);
 #pragma unroll
         for (int c = 1; c < BN / 32; ++c) b[c] = b[0];
+      };
+      for (int kb = 0; kb < kblocks; kb += 4) {
+        fetch(kb);
         if (!mbar_wait_warp(sf_empty + slot, sphase ^ 1u, p.err, kErrGemm8Scales)) { ok = false; break; }
         tc_fence_after();
         const uint32_t at = tmem_base + lanes + Cfg::kSfCol0 + slot * Cfg::kSfCols;
@@ -720,7 +726,7 @@ __global__ void __launch_bounds__(512, 1)
             any = true;
           }
           if ((kb & 3) == 0) {
-            if (!mbar_wait_cluster_warp(sf_full + slot, sphase, p.err, kErrGemm8Mma)) { ok = false; break; }
+            if (!mbar_wait_warp(sf_full + slot, sphase, p.err, kErrGemm8Mma)) { ok = false; break; }
           }
           if (!mbar_wait_warp(full + stage, phase, p.err, kErrGemm8Mma)) { ok = false; break; }
           tc_fence_after();
@@ -748,37 +754,52 @@ __global__ void __launch_bounds__(512, 1)
   } else if (warp < 8) {
     // ------------------------------------------------------------ scales -> TMEM
     if constexpr (KIND == kG8Gelu) reg_dealloc<56>();
+    // The words of a group of four K blocks are on their way a group ahead,
+    // across tiles, so that no slot waits for global memory.
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t sf_full0 = map_to_rank(sf_full, 0);
+    uint32_t a[4], b0, b4;
+    auto next_tile = [&](long long t) {
+      while (t < total && !pair_has_rows((int)(t / n_tiles))) t += n_pairs;
+      return t;
+    };
+    auto fetch = [&](long long t, int kb) {
+      if (t >= total) return;
+      const int mt = (int)(t / n_tiles), nt = (int)(t % n_tiles);
+      const uint8_t* wrow = p.w_scales + (long long)(2 * nt) * kblocks;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int row = mt * 256 + (int)rank * 128 + 32 * c + lane;
+        a[c] = row < p.M ? scale_word(p.a_scales + (long long)row * kblocks, kb, kblocks, p.a_words) : 0x7f7f7f7fu;
+      }
+      b0 = scale_word(wrow, kb, kblocks, p.w_words);
+      b4 = nt * 256 + 128 < p.N ? scale_word(wrow + kblocks, kb, kblocks, p.w_words) : 0x7f7f7f7fu;
+    };
     int slot = 0;
     uint32_t sphase = 0;
     bool ok = true;
-    for (long long t = pair; t < total && ok; t += n_pairs) {
-      const int mt = (int)(t / n_tiles), nt = (int)(t % n_tiles);
-      if (!pair_has_rows(mt)) continue;
-      const uint8_t* wrow0 = p.w_scales + (long long)(2 * nt) * kblocks;
-      const bool two = nt * 256 + 128 < p.N;
+    long long t = next_tile(pair);
+    fetch(t, 0);
+    while (t < total && ok) {
+      const long long after = next_tile(t + n_pairs);
       for (int kb = 0; kb < kblocks; kb += 4) {
-        uint32_t a[4], b[8];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int row = mt * 256 + (int)rank * 128 + 32 * c + lane;
-          a[c] = row < p.M ? scale_word(p.a_scales + (long long)row * kblocks, kb, kblocks) : 0x7f7f7f7fu;
-        }
-        b[0] = scale_word(wrow0, kb, kblocks);
-        b[4] = two ? scale_word(wrow0 + kblocks, kb, kblocks) : 0x7f7f7f7fu;
-#pragma unroll
-        for (int c = 1; c < 4; ++c) { b[c] = b[0]; b[4 + c] = b[4]; }
+        const uint32_t wa[4] = {a[0], a[1], a[2], a[3]};
+        const uint32_t wb[8] = {b0, b0, b0, b0, b4, b4, b4, b4};
+        if (kb + 4 < kblocks) fetch(t, kb + 4);
+        else fetch(after, 0);
         if (!mbar_wait_warp(sf_empty + slot, sphase ^ 1u, p.err, kErrGemm8Scales)) { ok = false; break; }
         tc_fence_after();
         const uint32_t at = tmem_base + lanes + Cfg::kSfCol0 + slot * Cfg::kSfCols;
-        tmem_st_words<4>(at, a);
-        tmem_st_words<8>(at + 4, b);
+        tmem_st_words<4>(at, wa);
+        tmem_st_words<8>(at + 4, wb);
         tmem_st_wait();
+        // TMEM alone is handed over, which the tcgen05 fences order; a release
+        // at cluster scope would wait for the loads above (22 us of 158)
         tc_fence_before();
-        mbar_arrive_cluster_release(sf_full0 + (uint32_t)(slot * sizeof(uint64_t)));
+        mbar_arrive_cluster_elect(sf_full0 + (uint32_t)(slot * sizeof(uint64_t)));
         if (++slot == SF) { slot = 0; sphase ^= 1u; }
       }
+      t = after;
     }
   } else {
     // ------------------------------------------------------------ epilogue

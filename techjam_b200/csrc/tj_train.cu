@@ -190,6 +190,8 @@ int gemm8_params(tj::Gemm8Params* p, const void* a, const uint8_t* as, const voi
   if (bias != nullptr && !aligned(bias, 16)) return fail(TJ_ERR_INVALID, "bias not 16-byte aligned");
   p->M = m; p->N = n; p->K = k;
   p->kblocks = blocks_of(k);
+  p->a_words = p->kblocks % 4 == 0 && aligned(as, 4);
+  p->w_words = p->kblocks % 4 == 0 && aligned(ws, 4);
   p->a_scales = as; p->w_scales = ws; p->bias = bias; p->mask = mask; p->err = err;
   return TJ_OK;
 }
