@@ -176,18 +176,41 @@ TJ_DEV uint32_t pack_bf162(float a, float b) {
 // 128-byte TMA swizzle; conflict-free for one piece per lane).
 TJ_DEV uint8_t* staged(uint8_t* buf, int lane, int j) { return buf + lane * 128 + ((j ^ (lane & 7)) << 4); }
 
-// GELU epilogue of one row's block of 128: h in 32 bits -> staged codes of
-// g = gelu(h) and of h, and their scale bytes (rows that are not valid: zeros).
+// gelu(x) = max(x, 0) - |x| erfc(|x| / sqrt 2) / 2 for two values, erfc from
+// Abramowitz & Stegun 7.1.26 as in gelu_erf_x2 (nothing cancels for x < 0).
+// The SFU bounds this epilogue (8 cycles an operation and warp), so both
+// reciprocals come from that of the product: 1 / d0 = d1 / (d0 d1).
+TJ_DEV float2 gelu8_x2(float x0, float x1) {
+  constexpr float kP = 0.3275911f * 0.70710678118654752f;
+  const float d0 = fmaf(fabsf(x0), kP, 1.f), d1 = fmaf(fabsf(x1), kP, 1.f);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d0 * d1));
+  const uint64_t t = f32x2(r * d1, r * d0);
+  uint64_t q = ffma_x2(t, f32x2(0.5f * 1.061405429f, 0.5f * 1.061405429f), f32x2(-0.5f * 1.453152027f, -0.5f * 1.453152027f));
+  q = ffma_x2(t, q, f32x2(0.5f * 1.421413741f, 0.5f * 1.421413741f));
+  q = ffma_x2(t, q, f32x2(-0.5f * 0.284496736f, -0.5f * 0.284496736f));
+  q = ffma_x2(t, q, f32x2(0.5f * 0.254829592f, 0.5f * 0.254829592f));
+  const uint64_t y = fmul_x2(f32x2(x0, x1), f32x2(0.84932180028801904f, 0.84932180028801904f));  // sqrt(log2(e) / 2)
+  const float2 yy = f32x2_split(fmul_x2(y, y));
+  const float2 tail = f32x2_split(fmul_x2(fmul_x2(t, q), f32x2(fast_exp2(-yy.x), fast_exp2(-yy.y))));
+  return make_float2(fmaf(-fabsf(x0), tail.x, fmaxf(x0, 0.f)), fmaf(-fabsf(x1), tail.y, fmaxf(x1, 0.f)));
+}
+
+// GELU epilogue of N columns (a block of 128, or half of one) of one row: h in
+// 32 bits -> staged codes of g = gelu(h) and of h from 16-byte piece `piece0`
+// on, and the block's scale bytes (rows that are not valid: zeros).  join(a, b)
+// takes the maxima with the other half's.
 // gelu grows with h > 0 and its dip for h < 0 is 0.17 deep, which gelu(0.3)
 // exceeds: above that the largest |g| is gelu of the largest h, and only a
 // warp with a smaller one looks at every g.  Called by whole warps.
-TJ_DEV void gelu_pack_row(float (&h)[128], bool valid, uint8_t* bufg, uint8_t* bufh, int lane, uint32_t& gbyte,
-                          uint32_t& hbyte) {
+template <int N, typename Join>
+TJ_DEV void gelu_pack_row(float (&h)[N], bool valid, uint8_t* bufg, uint8_t* bufh, int piece0, int lane,
+                          uint32_t& gbyte, uint32_t& hbyte, Join&& join) {
   float hmax = 0.f, hpos = 0.f;
   auto maxima = [&] {
     float m[4] = {0.f, 0.f, 0.f, 0.f}, q[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 128; i += 8)
+    for (int i = 0; i < N; i += 8)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         m[k] = max3f(m[k], fabsf(h[i + 2 * k]), fabsf(h[i + 2 * k + 1]));
@@ -199,34 +222,37 @@ TJ_DEV void gelu_pack_row(float (&h)[128], bool valid, uint8_t* bufg, uint8_t* b
   maxima();
   if (__any_sync(0xffffffffu, hmax > 3.402823466e38f)) {  // infinities become NaN, which the maxima drop
 #pragma unroll
-    for (int i = 0; i < 128; ++i)
+    for (int i = 0; i < N; ++i)
       if (fabsf(h[i]) > 3.402823466e38f) h[i] = __int_as_float(0x7fffffff);
     maxima();
   }
-  float gmax = gelu_erf_x2(hpos, 0.f).x;
-  if (__any_sync(0xffffffffu, hpos < 0.3f)) {
+  join(hmax, hpos);
+  float gmax = gelu8_x2(hpos, 0.f).x;
+  if (__any_sync(0xffffffffu, hpos < 0.3f)) {  // the same in both halves' warps
 #pragma unroll
-    for (int i = 0; i < 128; i += 2) {
-      const float2 g = gelu_erf_x2(h[i], h[i + 1]);
+    for (int i = 0; i < N; i += 2) {
+      const float2 g = gelu8_x2(h[i], h[i + 1]);
       gmax = max3f(gmax, fabsf(g.x), fabsf(g.y));
     }
+    float same = gmax;
+    join(gmax, same);
   }
   gbyte = valid ? scale_byte(gmax) : 127u;
   hbyte = valid ? scale_byte(hmax) : 127u;
   const float ginv = scale_inv(gbyte), hinv = scale_inv(hbyte);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < N / 16; ++j) {
     uint32_t gw[4], hw[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float* v = h + 16 * j + 4 * i;
-      const float2 g0 = gelu_erf_x2(v[0], v[1]), g1 = gelu_erf_x2(v[2], v[3]);
+      const float2 g0 = gelu8_x2(v[0], v[1]), g1 = gelu8_x2(v[2], v[3]);
       gw[i] = e4m3x2<false>(g0.x, g0.y, ginv) | (e4m3x2<false>(g1.x, g1.y, ginv) << 16);
       hw[i] = e4m3x2<false>(v[0], v[1], hinv) | (e4m3x2<false>(v[2], v[3], hinv) << 16);
     }
-    *reinterpret_cast<uint4*>(staged(bufg, lane, j)) =
+    *reinterpret_cast<uint4*>(staged(bufg, lane, piece0 + j)) =
         valid ? make_uint4(gw[0], gw[1], gw[2], gw[3]) : make_uint4(0, 0, 0, 0);
-    *reinterpret_cast<uint4*>(staged(bufh, lane, j)) =
+    *reinterpret_cast<uint4*>(staged(bufh, lane, piece0 + j)) =
         valid ? make_uint4(hw[0], hw[1], hw[2], hw[3]) : make_uint4(0, 0, 0, 0);
   }
 }
@@ -562,7 +588,7 @@ __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
         if (store) {
           if (lane == 0) bulk_wait_read<2>();
           __syncwarp();
-          gelu_pack_row(h, valid, bufg, bufh, lane, gbyte, hbyte);
+          gelu_pack_row<128>(h, valid, bufg, bufh, 0, lane, gbyte, hbyte, [](float&, float&) {});
           fence_async_smem();
           __syncwarp();
           if (lane == 0) {
@@ -603,16 +629,19 @@ template <int KIND>
 struct Gemm8PairCfg {
   static constexpr int kBN = 256;
   static constexpr int kStageBytes = 2 * 128 * 128;
-  static constexpr int kBufs = 2;
-  static constexpr int kStagingBytes = 8 * kBufs * 4096;
+  // kG8Gelu: 16 epilogue warps of 64 columns, each two sharing a block and its
+  // staging (with 8 of 128 columns the SFU and FMA latencies showed: 64 us
+  // for 16384 x 2048 x 512); else 8 warps of 128 columns
+  static constexpr int kEpiWarps = KIND == kG8Gelu ? 16 : 8;
+  static constexpr int kStagingBytes = 64 * 1024;
   static constexpr int kStages = 5;
   static constexpr int kAcc1 = 224;   // first column of buffer 1
   static constexpr int kSfCol0 = 480;
   static constexpr int kSfSlots = 2;
   static constexpr int kSfCols = 12;  // 4 for A's 128 rows, 8 for W's 256
-  static constexpr int kThreads = 512;
-  static constexpr int kRegLaunch = 128;  // kG8Gelu: warpgroups with 56 + 56 + 2 * 200
-  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kStagingBytes + 512;
+  static constexpr int kThreads = 256 + 32 * kEpiWarps;
+  static constexpr int kRegLaunch = KIND == kG8Gelu ? 80 : 128;  // kG8Gelu: warpgroups with 40 + 56 + 4 * 96
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kStagingBytes + 256;
   static_assert(kSmemBytes <= 232448, "shared memory");
 };
 
@@ -629,7 +658,7 @@ TJ_DEV void umma_mx8_pair_elect(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
 }
 
 template <int KIND>
-__global__ void __launch_bounds__(512, 1)
+__global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
     gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                       const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ CUtensorMap tmAux,
                       const Gemm8Params p) {
@@ -654,7 +683,7 @@ __global__ void __launch_bounds__(512, 1)
   const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(acc_full + i, 1); mbar_init(acc_empty + i, 16); }
+    for (int i = 0; i < 2; ++i) { mbar_init(acc_full + i, 1); mbar_init(acc_empty + i, 2 * Cfg::kEpiWarps); }
     mbar_init(shared_free, 8);
     for (int i = 0; i < SF; ++i) { mbar_init(sf_full + i, 8); mbar_init(sf_empty + i, 1); }
     fence_mbar_init();
@@ -679,7 +708,7 @@ __global__ void __launch_bounds__(512, 1)
   };
 
   if (warp < 4) {
-    if constexpr (KIND == kG8Gelu) reg_dealloc<56>();
+    if constexpr (KIND == kG8Gelu) reg_dealloc<40>();
     if (warp == 0) {
       // ---------------------------------------------------------- TMA producer
       if (lane == 0) { tma_prefetch_desc(&tmA); tma_prefetch_desc(&tmW); }
@@ -803,9 +832,12 @@ __global__ void __launch_bounds__(512, 1)
     }
   } else {
     // ------------------------------------------------------------ epilogue
-    if constexpr (KIND == kG8Gelu) reg_alloc<200>();
-    const int ew = warp - 8, quarter = warp & 3, half = ew >> 2;
-    uint8_t* bufs = staging + ew * Cfg::kBufs * 4096;
+    if constexpr (KIND == kG8Gelu) reg_alloc<96>();
+    const int ew = warp - 8, quarter = warp & 3;
+    constexpr int kGroups = Cfg::kEpiWarps / 4, kCW = 256 / kGroups;
+    const int cg = ew >> 2;  // column group
+    // two 4 KB buffers a warp, or a pair of warps
+    uint8_t* bufs = staging + (KIND == kG8Gelu ? 4 * (cg >> 1) + quarter : ew) * 8192;
     const uint32_t acc_empty0 = map_to_rank(acc_empty, 0), shared_free0 = map_to_rank(shared_free, 0);
     uint32_t used = 0;  // staging buffers used so far
     int abuf = 0;
@@ -815,7 +847,7 @@ __global__ void __launch_bounds__(512, 1)
       const int mt = (int)(t / n_tiles), nt = (int)(t % n_tiles);
       const bool live = pair_has_rows(mt);
       const int row0 = mt * 256 + (int)rank * 128 + quarter * 32;
-      const int col0 = nt * 256 + half * 128;
+      const int col0 = nt * 256 + cg * kCW;
       const int row = row0 + lane;
       const bool valid = row < p.M && (p.mask == nullptr || __ldg(p.mask + row) != 0);
       auto wait_acc = [&] {
@@ -823,7 +855,7 @@ __global__ void __launch_bounds__(512, 1)
         tc_fence_after();
         return ok;
       };
-      auto acc_addr = [&] { return tmem_base + ((uint32_t)(quarter * 32) << 16) + abuf * Cfg::kAcc1 + half * 128; };
+      auto acc_addr = [&] { return tmem_base + ((uint32_t)(quarter * 32) << 16) + abuf * Cfg::kAcc1 + cg * kCW; };
       auto free_shared = [&] {
         tc_fence_before();
         mbar_arrive_cluster_elect(shared_free0);
@@ -834,73 +866,77 @@ __global__ void __launch_bounds__(512, 1)
         if (++abuf == 2) { abuf = 0; aphase ^= 1u; }
       };
       if constexpr (KIND == kG8Gelu) {
-        float h[128];
+        float h[64];
 #pragma unroll
-        for (int i = 0; i < 128; ++i) h[i] = 0.f;
+        for (int i = 0; i < 64; ++i) h[i] = 0.f;
         if (live) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) add_bias32(h + 32 * c, p.bias, col0 + 32 * c, p.N);
           for (int kb = 0; kb < kblocks; kb += kChunk) {
             if (!wait_acc()) break;
-            // buffer 0 shares its last 32 columns, buffer 1 its first: both
-            // are this warp's piece 3 or 0, if they are in its half at all
             const uint32_t taddr = acc_addr();
-            const bool mine = half == (abuf ^ 1);
-            if (mine) {
-              uint32_t r[32];
-              if (abuf == 0) {
-                tmem_ld32(taddr + 96, r);
-                tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) h[96 + i] += __uint_as_float(r[i]);
-              } else {
-                tmem_ld32(taddr, r);
-                tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) h[i] += __uint_as_float(r[i]);
-              }
-              free_shared();
-            }
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              if (mine && c == (abuf == 0 ? 3 : 0)) continue;  // warp-uniform
-              uint32_t r[32];
-              tmem_ld32(taddr + 32 * c, r);
-              tmem_ld_wait();
+            // buffer 0 shares its last 32 columns (group 3's second piece),
+            // buffer 1 its first (group 0's first)
+            const bool swap = abuf == 0 && cg == 3;
+            const bool mine = swap || (abuf == 1 && cg == 0);
+            uint32_t r[32];
+            auto add = [&](int c) {
 #pragma unroll
               for (int i = 0; i < 32; ++i) h[32 * c + i] += __uint_as_float(r[i]);
-            }
+            };
+            tmem_ld32(taddr + (swap ? 32 : 0), r);
+            tmem_ld_wait();
+            if (mine) free_shared();
+            if (swap) add(1); else add(0);
+            tmem_ld32(taddr + (swap ? 0 : 32), r);
+            tmem_ld_wait();
             free_acc();
+            if (swap) add(0); else add(1);
           }
           if (!ok) break;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) add_bias32(h + 32 * c, p.bias, col0 + 32 * c, p.N);
         }
-        if (row0 < p.M && col0 < p.N) {
+        // the two warps of a block meet at a barrier of their own, and
+        // exchange their maxima in the staging before the codes fill it
+        float2* other = reinterpret_cast<float2*>(bufs);
+        const int bar_id = 1 + (cg >> 1) * 4 + quarter;
+        auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(bar_id) : "memory"); };
+        const int cb = nt * 256 + (cg >> 1) * 128;  // the block's first column
+        if (row0 < p.M && cb < p.N) {
           uint32_t gbyte, hbyte;
-          if (lane == 0) bulk_wait_read<0>();
-          __syncwarp();
-          gelu_pack_row(h, valid, bufs, bufs + 4096, lane, gbyte, hbyte);
+          if ((cg & 1) == 0 && lane == 0) bulk_wait_read<0>();  // before the first meeting: the staging is free
+          gelu_pack_row<64>(h, valid, bufs, bufs + 4096, 4 * (cg & 1), lane, gbyte, hbyte, [&](float& a, float& b) {
+            meet();
+            other[32 * (cg & 1) + lane] = make_float2(a, b);
+            meet();
+            const float2 o = other[32 * ((cg & 1) ^ 1) + lane];
+            meet();
+            a = fmaxf(a, o.x);
+            b = fmaxf(b, o.y);
+          });
           fence_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_2d(&tmOut, bufs, col0, row0);
-            tma_store_2d(&tmAux, bufs + 4096, col0, row0);
-            bulk_commit();
-          }
-          if (row < p.M) {
-            const long long s = (long long)row * n_blocks(p.N) + col0 / kBlk;
-            p.g_scales[s] = (uint8_t)gbyte;
-            p.h_scales[s] = (uint8_t)hbyte;
+          meet();
+          if ((cg & 1) == 0) {
+            if (lane == 0) {
+              tma_store_2d(&tmOut, bufs, cb, row0);
+              tma_store_2d(&tmAux, bufs + 4096, cb, row0);
+              bulk_commit();
+            }
+            if (row < p.M) {
+              const long long s = (long long)row * n_blocks(p.N) + cb / kBlk;
+              p.g_scales[s] = (uint8_t)gbyte;
+              p.h_scales[s] = (uint8_t)hbyte;
+            }
           }
         }
       } else {
         if (live && !wait_acc()) break;
         const int cur = abuf;
         const uint32_t taddr = acc_addr();
-        const bool mine = half == (cur ^ 1);
+        const bool mine = cg == (cur ^ 1);
         // two 64-column pieces, the one with the shared columns first
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const int piece = cur == 0 && half == 1 ? 1 - q : q;
+          const int piece = cur == 0 && cg == 1 ? 1 - q : q;
           const int col = col0 + 64 * piece;
           uint32_t r[2][32];
           if (live) {
