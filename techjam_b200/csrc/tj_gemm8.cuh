@@ -180,9 +180,10 @@ TJ_DEV uint8_t* staged(uint8_t* buf, int lane, int j) { return buf + lane * 128 
 // Abramowitz & Stegun 7.1.26 as in gelu_erf_x2 (nothing cancels for x < 0).
 // The SFU bounds this epilogue (8 cycles an operation and warp), so both
 // reciprocals come from that of the product: 1 / d0 = d1 / (d0 d1).
-TJ_DEV float2 gelu8_x2(float x0, float x1) {
+TJ_DEV uint64_t gelu8_x2(uint64_t x) {
   constexpr float kP = 0.3275911f * 0.70710678118654752f;
-  const float d0 = fmaf(fabsf(x0), kP, 1.f), d1 = fmaf(fabsf(x1), kP, 1.f);
+  const float2 v = f32x2_split(x);
+  const float d0 = fmaf(fabsf(v.x), kP, 1.f), d1 = fmaf(fabsf(v.y), kP, 1.f);
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d0 * d1));
   const uint64_t t = f32x2(r * d1, r * d0);
@@ -190,48 +191,56 @@ TJ_DEV float2 gelu8_x2(float x0, float x1) {
   q = ffma_x2(t, q, f32x2(0.5f * 1.421413741f, 0.5f * 1.421413741f));
   q = ffma_x2(t, q, f32x2(-0.5f * 0.284496736f, -0.5f * 0.284496736f));
   q = ffma_x2(t, q, f32x2(0.5f * 0.254829592f, 0.5f * 0.254829592f));
-  const uint64_t y = fmul_x2(f32x2(x0, x1), f32x2(0.84932180028801904f, 0.84932180028801904f));  // sqrt(log2(e) / 2)
+  const uint64_t y = fmul_x2(x, f32x2(0.84932180028801904f, 0.84932180028801904f));  // sqrt(log2(e) / 2)
   const float2 yy = f32x2_split(fmul_x2(y, y));
   const float2 tail = f32x2_split(fmul_x2(fmul_x2(t, q), f32x2(fast_exp2(-yy.x), fast_exp2(-yy.y))));
-  return make_float2(fmaf(-fabsf(x0), tail.x, fmaxf(x0, 0.f)), fmaf(-fabsf(x1), tail.y, fmaxf(x1, 0.f)));
+  return f32x2(fmaf(-fabsf(v.x), tail.x, fmaxf(v.x, 0.f)), fmaf(-fabsf(v.y), tail.y, fmaxf(v.y, 0.f)));
+}
+TJ_DEV uint32_t e4m3_pair(uint64_t x, uint64_t inv) {  // no infinities
+  uint16_t r;
+  const float2 v = f32x2_split(fmul_x2(x, inv));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(v.y), "f"(v.x));
+  return r;
 }
 
 // GELU epilogue of N columns (a block of 128, or half of one) of one row: h in
-// 32 bits -> staged codes of g = gelu(h) and of h from 16-byte piece `piece0`
-// on, and the block's scale bytes (rows that are not valid: zeros).  join(a, b)
-// takes the maxima with the other half's.
+// 32 bits, two to a word -> staged codes of g = gelu(h) and of h from 16-byte
+// piece `piece0` on, and the block's scale bytes (rows that are not valid:
+// zeros).  join(a, b) takes the maxima with the other half's.
 // gelu grows with h > 0 and its dip for h < 0 is 0.17 deep, which gelu(0.3)
 // exceeds: above that the largest |g| is gelu of the largest h, and only a
 // warp with a smaller one looks at every g.  Called by whole warps.
 template <int N, typename Join>
-TJ_DEV void gelu_pack_row(float (&h)[N], bool valid, uint8_t* bufg, uint8_t* bufh, int piece0, int lane,
+TJ_DEV void gelu_pack_row(uint64_t (&h)[N / 2], bool valid, uint8_t* bufg, uint8_t* bufh, int piece0, int lane,
                           uint32_t& gbyte, uint32_t& hbyte, Join&& join) {
   float hmax = 0.f, hpos = 0.f;
   auto maxima = [&] {
     float m[4] = {0.f, 0.f, 0.f, 0.f}, q[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < N; i += 8)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        m[k] = max3f(m[k], fabsf(h[i + 2 * k]), fabsf(h[i + 2 * k + 1]));
-        q[k] = max3f(q[k], h[i + 2 * k], h[i + 2 * k + 1]);
-      }
+    for (int i = 0; i < N / 2; ++i) {
+      const float2 v = f32x2_split(h[i]);
+      m[i & 3] = max3f(m[i & 3], fabsf(v.x), fabsf(v.y));
+      q[i & 3] = max3f(q[i & 3], v.x, v.y);
+    }
     hmax = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
     hpos = fmaxf(fmaxf(q[0], q[1]), fmaxf(q[2], q[3]));
   };
   maxima();
   if (__any_sync(0xffffffffu, hmax > 3.402823466e38f)) {  // infinities become NaN, which the maxima drop
+    const float nan = __int_as_float(0x7fffffff);
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (fabsf(h[i]) > 3.402823466e38f) h[i] = __int_as_float(0x7fffffff);
+    for (int i = 0; i < N / 2; ++i) {
+      const float2 v = f32x2_split(h[i]);
+      h[i] = f32x2(fabsf(v.x) > 3.402823466e38f ? nan : v.x, fabsf(v.y) > 3.402823466e38f ? nan : v.y);
+    }
     maxima();
   }
   join(hmax, hpos);
-  float gmax = gelu8_x2(hpos, 0.f).x;
+  float gmax = f32x2_split(gelu8_x2(f32x2(hpos, 0.f))).x;
   if (__any_sync(0xffffffffu, hpos < 0.3f)) {  // the same in both halves' warps
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const float2 g = gelu8_x2(h[i], h[i + 1]);
+    for (int i = 0; i < N / 2; ++i) {
+      const float2 g = f32x2_split(gelu8_x2(h[i]));
       gmax = max3f(gmax, fabsf(g.x), fabsf(g.y));
     }
     float same = gmax;
@@ -239,22 +248,36 @@ TJ_DEV void gelu_pack_row(float (&h)[N], bool valid, uint8_t* bufg, uint8_t* buf
   }
   gbyte = valid ? scale_byte(gmax) : 127u;
   hbyte = valid ? scale_byte(hmax) : 127u;
-  const float ginv = scale_inv(gbyte), hinv = scale_inv(hbyte);
+  const uint64_t ginv = f32x2(scale_inv(gbyte), scale_inv(gbyte)), hinv = f32x2(scale_inv(hbyte), scale_inv(hbyte));
 #pragma unroll
   for (int j = 0; j < N / 16; ++j) {
     uint32_t gw[4], hw[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float* v = h + 16 * j + 4 * i;
-      const float2 g0 = gelu8_x2(v[0], v[1]), g1 = gelu8_x2(v[2], v[3]);
-      gw[i] = e4m3x2<false>(g0.x, g0.y, ginv) | (e4m3x2<false>(g1.x, g1.y, ginv) << 16);
-      hw[i] = e4m3x2<false>(v[0], v[1], hinv) | (e4m3x2<false>(v[2], v[3], hinv) << 16);
+      const uint64_t v0 = h[8 * j + 2 * i], v1 = h[8 * j + 2 * i + 1];
+      gw[i] = __byte_perm(e4m3_pair(gelu8_x2(v0), ginv), e4m3_pair(gelu8_x2(v1), ginv), 0x5410);
+      hw[i] = __byte_perm(e4m3_pair(v0, hinv), e4m3_pair(v1, hinv), 0x5410);
     }
     *reinterpret_cast<uint4*>(staged(bufg, lane, piece0 + j)) =
         valid ? make_uint4(gw[0], gw[1], gw[2], gw[3]) : make_uint4(0, 0, 0, 0);
     *reinterpret_cast<uint4*>(staged(bufh, lane, piece0 + j)) =
         valid ? make_uint4(hw[0], hw[1], hw[2], hw[3]) : make_uint4(0, 0, 0, 0);
   }
+}
+// h = the bias of columns col0.. (zeros past n), and h += 32 accumulator columns.
+template <int N>
+TJ_DEV void bias_pairs(uint64_t (&h)[N / 2], const float* bias, int col0, int n) {
+#pragma unroll
+  for (int j = 0; j < N / 4; ++j) {
+    float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (bias != nullptr && col0 + 4 * j < n) b = __ldg(reinterpret_cast<const float4*>(bias + col0) + j);
+    h[2 * j] = f32x2(b.x, b.y);
+    h[2 * j + 1] = f32x2(b.z, b.w);
+  }
+}
+TJ_DEV void add_pairs(uint64_t* h, const uint32_t (&r)[32]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) h[i] = fadd_x2(h[i], f32x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])));
 }
 
 // Adds the bias of columns col0.. (zeros past n) to 32 values.
@@ -565,9 +588,8 @@ __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
         uint32_t gbyte = 127u, hbyte = 127u;
         uint8_t* bufg = bufs + (used % Cfg::kBufs) * 4096;
         uint8_t* bufh = bufs + ((used + 1) % Cfg::kBufs) * 4096;
-        float h[128];
-#pragma unroll
-        for (int i = 0; i < 128; ++i) h[i] = 0.f;
+        uint64_t h[64];
+        bias_pairs<128>(h, p.bias, col0, p.N);
         if (live) {
           for (int kb = 0; kb < kblocks; kb += kChunk) {
             if (!wait_acc()) break;
@@ -576,14 +598,11 @@ __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
               uint32_t r[32];
               tmem_ld32(taddr + abuf * BN + 32 * c, r);
               tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) h[32 * c + i] += __uint_as_float(r[i]);
+              add_pairs(h + 16 * c, r);
             }
             free_acc();
           }
           if (!ok) break;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) add_bias32(h + 32 * c, p.bias, col0 + 32 * c, p.N);
         }
         if (store) {
           if (lane == 0) bulk_wait_read<2>();
@@ -866,12 +885,9 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
         if (++abuf == 2) { abuf = 0; aphase ^= 1u; }
       };
       if constexpr (KIND == kG8Gelu) {
-        float h[64];
-#pragma unroll
-        for (int i = 0; i < 64; ++i) h[i] = 0.f;
+        uint64_t h[32];
+        bias_pairs<64>(h, p.bias, col0, p.N);
         if (live) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) add_bias32(h + 32 * c, p.bias, col0 + 32 * c, p.N);
           for (int kb = 0; kb < kblocks; kb += kChunk) {
             if (!wait_acc()) break;
             const uint32_t taddr = acc_addr();
@@ -880,18 +896,14 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
             const bool swap = abuf == 0 && cg == 3;
             const bool mine = swap || (abuf == 1 && cg == 0);
             uint32_t r[32];
-            auto add = [&](int c) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) h[32 * c + i] += __uint_as_float(r[i]);
-            };
             tmem_ld32(taddr + (swap ? 32 : 0), r);
             tmem_ld_wait();
             if (mine) free_shared();
-            if (swap) add(1); else add(0);
+            if (swap) add_pairs(h + 16, r); else add_pairs(h, r);
             tmem_ld32(taddr + (swap ? 0 : 32), r);
             tmem_ld_wait();
             free_acc();
-            if (swap) add(0); else add(1);
+            if (swap) add_pairs(h, r); else add_pairs(h + 16, r);
           }
           if (!ok) break;
         }
