@@ -178,6 +178,7 @@ def poly_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, exact_pref
 # ---------------------------------------------------------------- training and 8-bit activations
 
 _DTYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_F32 = (torch.float32,)
 
 
 class Act8(NamedTuple):
@@ -201,33 +202,48 @@ class LayerNormOut(NamedTuple):
     x8: Optional[Act8]    # 8-bit copy of the input, when asked for
 
 
-def _run(device: torch.device, name: str, *args) -> None:
-    """Call an entry point on the device's current stream."""
-    if torch.cuda.current_device() == device.index:
-        _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+_E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+# the handle and the index alone: the public forms build objects on each call
+_stream_of, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+_entries: dict = {}
+
+
+def _run(index: int, name: str, *args) -> None:
+    """Call an entry point on the current stream of CUDA device ``index``."""
+    entry = _entries.get(name)
+    if entry is None:
+        entry = _entries[name] = getattr(_lib.load(), name)
+    if _current_device() == index:
+        status = entry(*args, _stream_of(index))
     else:
-        with torch.cuda.device(device):
-            _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+        with torch.cuda.device(index):
+            status = entry(*args, _stream_of(index))
+    if status:
+        _lib.check(status)
 
 
-def _matrix(t: torch.Tensor, what: str, dtypes, shape=None, device=None) -> None:
-    if t.device.type != "cuda" or not t.is_contiguous():
+def _matrix(t: torch.Tensor, what: str, dtypes, shape=None, index: Optional[int] = None) -> int:
+    """Check an operand ([rows, cols], or the given shape) and return its CUDA device's index."""
+    at = t.get_device()
+    if (at >= 0 and t.is_contiguous() and t.dtype in dtypes and (index is None or at == index)
+            and (t.shape == shape if shape is not None else t.dim() == 2 and t.shape[1] > 0)):
+        return at
+    if at < 0 or not t.is_contiguous():
         raise ValueError(f"{what}: techjam_b200.ops needs contiguous CUDA tensors")
     if t.dtype not in dtypes:
         raise ValueError(f"{what}: dtype {t.dtype}, need one of {', '.join(map(str, dtypes))}")
-    if t.dim() != 2 if shape is None else tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{what}: shape {tuple(t.shape)}, need {'[rows, cols]' if shape is None else tuple(shape)}")
+    if index is not None and at != index:
+        raise ValueError(f"{what}: on {t.device}, need cuda:{index}")
     if t.dim() == 2 and t.shape[1] == 0:
         raise ValueError(f"{what}: no columns")
-    if device is not None and t.device != device:
-        raise ValueError(f"{what}: on {t.device}, need {device}")
+    raise ValueError(f"{what}: shape {tuple(t.shape)}, need {'[rows, cols]' if shape is None else tuple(shape)}")
 
 
-def _row_mask(mask: Optional[torch.Tensor], rows: int, device):
+def _row_mask(mask: Optional[torch.Tensor], rows: int, index: int):
     if mask is None:
         return None
-    if mask.device != device or not mask.is_contiguous() or mask.dtype != torch.bool or mask.numel() != rows:
-        raise ValueError(f"mask must be a contiguous bool tensor with one element per row ({rows}) on {device}")
+    if (mask.get_device() != index or not mask.is_contiguous() or mask.dtype != torch.bool or mask.numel() != rows):
+        raise ValueError(f"mask must be a contiguous bool tensor with one element per row ({rows}) on cuda:{index}")
     return mask.data_ptr()
 
 
@@ -235,36 +251,42 @@ def _blocks(n: int) -> int:
     return (n + 127) // 128
 
 
-def _check8(a, what: str, blocks, device=None) -> None:
-    _matrix(a.codes, f"{what} codes", (torch.float8_e4m3fn,), device=device)
-    _matrix(a.scales, f"{what} scales", (torch.float8_e8m0fnu,), blocks(*a.codes.shape), a.codes.device)
-
-
-def _check_act(a: Act8, what: str, device=None) -> None:
+def _check_act(a: Act8, what: str, index: Optional[int] = None):
+    """Check an 8-bit activation; (device index, rows, cols)."""
     if not isinstance(a, Act8):
         raise ValueError(f"{what} must be an Act8")
-    _check8(a, what, lambda r, c: (r, _blocks(c)), device)
+    index = _matrix(a.codes, what, (_E4M3,), None, index)
+    rows, cols = a.codes.shape
+    _matrix(a.scales, what, (_E8M0,), (rows, _blocks(cols)), index)
+    return index, rows, cols
 
 
 def _new_act(rows: int, cols: int, device, dtype) -> Act8:
-    return Act8(torch.empty(rows, cols, dtype=torch.float8_e4m3fn, device=device),
-                torch.empty(rows, _blocks(cols), dtype=torch.float8_e8m0fnu, device=device), dtype)
+    return Act8(torch.empty(rows, cols, dtype=_E4M3, device=device),
+                torch.empty(rows, _blocks(cols), dtype=_E8M0, device=device), dtype)
 
 
 _err_words: dict = {}
 
 
-def _err_word(device: torch.device) -> torch.Tensor:
+def _err_word(index: int) -> torch.Tensor:
     """The device's error word of the operators that wait inside a kernel
     (one per device, kept; first used outside a stream capture)."""
-    word = _err_words.get(device.index)
+    word = _err_words.get(index)
     if word is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("call this operator once on the device before capturing it")
-        word = torch.zeros(1, dtype=torch.int32, device=device)
-        torch.cuda.current_stream(device).synchronize()
-        word = _err_words.setdefault(device.index, word)
+        word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
+        torch.cuda.current_stream(index).synchronize()
+        word = _err_words.setdefault(index, word)
     return word
+
+
+def _err_ptr(err: Optional[torch.Tensor], index: int) -> int:
+    if err is None:
+        return _err_word(index).data_ptr()
+    _matrix(err, "err", (torch.int32,), (1,), index)
+    return err.data_ptr()
 
 
 def device_error(device=None) -> int:
@@ -275,7 +297,7 @@ def device_error(device=None) -> int:
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
     torch.cuda.synchronize(device)
-    word = _err_word(device)
+    word = _err_word(device.index)
     code = int(word.item())
     if code:
         word.zero_()
@@ -285,39 +307,38 @@ def device_error(device=None) -> int:
 def checkpoint8(x: torch.Tensor, mask: Optional[torch.Tensor] = None) -> Act8:
     """x [rows, cols] (fp32, fp16 or bf16) into 8 bits.  A block's codes depend
     on its values alone; infinities and NaN become NaN."""
-    _matrix(x, "x", _DTYPES)
+    index = _matrix(x, "x", _DTYPES)
     rows, cols = x.shape
+    mptr = _row_mask(mask, rows, index)
     out = _new_act(rows, cols, x.device, x.dtype)
-    _run(x.device, "tj_act8_pack", x.data_ptr(), _DTYPES[x.dtype], rows, cols, _row_mask(mask, rows, x.device),
-         out.codes.data_ptr(), out.scales.data_ptr())
+    _run(index, "tj_act8_pack", x.data_ptr(), _DTYPES[x.dtype], rows, cols, mptr, out.codes.data_ptr(),
+         out.scales.data_ptr())
     return out
 
 
 def restore8(a: Act8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """The values of an 8-bit activation: exact in fp32 and bf16 within their
     normal range, rounded in fp16; beyond a type's range its largest value."""
-    _check_act(a, "a")
+    index, rows, cols = _check_act(a, "a")
     dtype = a.dtype if dtype is None else dtype
     if dtype not in _DTYPES:
         raise ValueError(f"dtype {dtype}, need one of {', '.join(map(str, _DTYPES))}")
-    rows, cols = a.codes.shape
     out = torch.empty(rows, cols, dtype=dtype, device=a.codes.device)
-    _run(out.device, "tj_act8_unpack", a.codes.data_ptr(), a.scales.data_ptr(), rows, cols, out.data_ptr(),
-         _DTYPES[dtype])
+    _run(index, "tj_act8_unpack", a.codes.data_ptr(), a.scales.data_ptr(), rows, cols, out.data_ptr(), _DTYPES[dtype])
     return out
 
 
 def pack_weight8(w: torch.Tensor, transpose: bool = False) -> Weight8:
     """A weight [n, k] (fp32, fp16 or bf16) into 8 bits, or its transpose (for
     the product that takes a gradient back through the layer)."""
-    _matrix(w, "w", _DTYPES)
+    index = _matrix(w, "w", _DTYPES)
     n, k = w.shape
     if n == 0:
         raise ValueError("w: no rows")
     r, c = (k, n) if transpose else (n, k)
-    out = Weight8(torch.empty(r, c, dtype=torch.float8_e4m3fn, device=w.device),
-                  torch.empty(_blocks(r), _blocks(c), dtype=torch.float8_e8m0fnu, device=w.device))
-    _run(w.device, "tj_weight8_pack", w.data_ptr(), _DTYPES[w.dtype], n, k, int(transpose), out.codes.data_ptr(),
+    out = Weight8(torch.empty(r, c, dtype=_E4M3, device=w.device),
+                  torch.empty(_blocks(r), _blocks(c), dtype=_E8M0, device=w.device))
+    _run(index, "tj_weight8_pack", w.data_ptr(), _DTYPES[w.dtype], n, k, int(transpose), out.codes.data_ptr(),
          out.scales.data_ptr())
     return out
 
@@ -325,29 +346,52 @@ def pack_weight8(w: torch.Tensor, transpose: bool = False) -> Weight8:
 def layernorm_train(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, mask: Optional[torch.Tensor] = None,
                     eps: float = 1e-5, out_dtype: torch.dtype = torch.float16,
                     checkpoint: bool = False) -> LayerNormOut:
-    """LayerNorm of x [rows, d] (fp32, fp16 or bf16) that keeps mean and 1/std
-    for ``layernorm_backward``.  ``out_dtype`` torch.float8_e4m3fn gives y as
-    an Act8; ``checkpoint`` also returns an 8-bit copy of x."""
-    _matrix(x, "x", _DTYPES)
+    """LayerNorm of x [rows, d] (fp32, fp16 or bf16; d <= 4096) that keeps mean
+    and 1/std for ``layernorm_backward``.  ``out_dtype`` torch.float8_e4m3fn
+    gives y as an Act8; ``checkpoint`` also returns an 8-bit copy of x."""
+    index = _matrix(x, "x", _DTYPES)
     rows, d = x.shape
-    for t, what in ((weight, "weight"), (bias, "bias")):
-        _matrix(t, what, (torch.float32,), (d,), x.device)
-    mptr = _row_mask(mask, rows, x.device)
-    if out_dtype == torch.float8_e4m3fn:
-        y = _new_act(rows, d, x.device, x.dtype)
+    _matrix(weight, "weight", _F32, (d,), index)
+    _matrix(bias, "bias", _F32, (d,), index)
+    mptr = _row_mask(mask, rows, index)
+    dev = x.device
+    if out_dtype == _E4M3:
+        y = _new_act(rows, d, dev, x.dtype)
         yp, ys, yd = y.codes.data_ptr(), y.scales.data_ptr(), _lib.E4M3
     elif out_dtype in _DTYPES:
-        y = torch.empty(rows, d, dtype=out_dtype, device=x.device)
+        y = torch.empty(rows, d, dtype=out_dtype, device=dev)
         yp, ys, yd = y.data_ptr(), None, _DTYPES[out_dtype]
     else:
         raise ValueError(f"out_dtype {out_dtype} not supported")
-    stats = torch.empty(2, rows, dtype=torch.float32, device=x.device)
-    x8 = _new_act(rows, d, x.device, x.dtype) if checkpoint else None
-    mean, rstd = stats.unbind(0)
-    _run(x.device, "tj_layernorm_train", x.data_ptr(), _DTYPES[x.dtype], weight.data_ptr(), bias.data_ptr(), rows, d,
-         float(eps), mptr, yp, yd, ys, mean.data_ptr(), rstd.data_ptr(), x8.codes.data_ptr() if checkpoint else None,
+    mean = torch.empty(rows, dtype=torch.float32, device=dev)
+    rstd = torch.empty(rows, dtype=torch.float32, device=dev)
+    x8 = _new_act(rows, d, dev, x.dtype) if checkpoint else None
+    _run(index, "tj_layernorm_train", x.data_ptr(), _DTYPES[x.dtype], weight.data_ptr(), bias.data_ptr(), rows, d, eps,
+         mptr, yp, yd, ys, mean.data_ptr(), rstd.data_ptr(), x8.codes.data_ptr() if checkpoint else None,
          x8.scales.data_ptr() if checkpoint else None)
     return LayerNormOut(y, mean, rstd, x8)
+
+
+_workspace_sizes: dict = {}
+
+
+def _workspace(name: str, device: torch.device, *sizes: int):
+    """A fresh workspace from torch's allocator (so that calls on different
+    streams, or captured into different graphs, never share one), its address
+    and size; only the size that a shape needs is kept."""
+    key = (name, device.index, sizes)
+    n = _workspace_sizes.get(key)
+    if n is None:
+        nbytes = ctypes.c_size_t()
+        with torch.cuda.device(device):
+            _lib.call(name, *sizes, ctypes.byref(nbytes))
+        if len(_workspace_sizes) >= 4096:
+            _workspace_sizes.clear()
+        n = _workspace_sizes[key] = int(nbytes.value)
+    if n == 0:
+        return None, None, 0
+    ws = torch.empty(n, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr(), n
 
 
 def layernorm_backward(dy: torch.Tensor, x, weight: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
@@ -355,89 +399,72 @@ def layernorm_backward(dy: torch.Tensor, x, weight: torch.Tensor, mean: torch.Te
     """Gradients (dx, dweight, dbias) of LayerNorm for dy [rows, d] (fp32, fp16
     or bf16).  x: the input or its 8-bit copy; dx has its type.  ``resid_grad``
     (x's type) is the gradient of the branch around the norm, added to dx."""
-    _matrix(dy, "dy", _DTYPES)
-    rows, d = dy.shape
+    index = _matrix(dy, "dy", _DTYPES)
+    rows, d = shape = dy.shape
     if isinstance(x, Act8):
-        _check_act(x, "x", dy.device)
-        xt, xp, xs = x.codes, x.codes.data_ptr(), x.scales.data_ptr()
+        if _check_act(x, "x", index)[1:] != shape:
+            raise ValueError(f"x: shape {tuple(x.codes.shape)}, need {tuple(shape)}")
         if x.dtype not in _DTYPES:
             raise ValueError(f"x: dtype {x.dtype} not supported")
+        xp, xs = x.codes.data_ptr(), x.scales.data_ptr()
     else:
-        _matrix(x, "x", _DTYPES, device=dy.device)
-        xt, xp, xs = x, x.data_ptr(), None
-    if tuple(xt.shape) != (rows, d):
-        raise ValueError(f"x: shape {tuple(xt.shape)}, need {(rows, d)}")
-    _matrix(weight, "weight", (torch.float32,), (d,), dy.device)
-    for t, what in ((mean, "mean"), (rstd, "rstd")):
-        _matrix(t, what, (torch.float32,), (rows,), dy.device)
+        _matrix(x, "x", _DTYPES, shape, index)
+        xp, xs = x.data_ptr(), None
+    _matrix(weight, "weight", _F32, (d,), index)
+    _matrix(mean, "mean", _F32, (rows,), index)
+    _matrix(rstd, "rstd", _F32, (rows,), index)
+    rp = None
     if resid_grad is not None:
-        _matrix(resid_grad, "resid_grad", (x.dtype,), (rows, d), dy.device)
-    mptr = _row_mask(mask, rows, dy.device)
-    dx = torch.empty(rows, d, dtype=x.dtype, device=dy.device)
-    dwb = torch.empty(2, d, dtype=torch.float32, device=dy.device)
-    ws = _workspace("tj_layernorm_backward_workspace_bytes", dy.device, rows, d)
-    dweight, dbias = dwb.unbind(0)
-    _run(dy.device, "tj_layernorm_backward", dy.data_ptr(), _DTYPES[dy.dtype], xp, xs, weight.data_ptr(),
-         mean.data_ptr(), rstd.data_ptr(), rows, d, mptr, _ptr(resid_grad), dx.data_ptr(), _DTYPES[x.dtype],
-         dweight.data_ptr(), dbias.data_ptr(), ws.data_ptr(), ws.numel())
+        _matrix(resid_grad, "resid_grad", (x.dtype,), shape, index)
+        rp = resid_grad.data_ptr()
+    mptr = _row_mask(mask, rows, index)
+    dev = dy.device
+    dx = torch.empty(rows, d, dtype=x.dtype, device=dev)
+    dweight = torch.empty(d, dtype=torch.float32, device=dev)
+    dbias = torch.empty(d, dtype=torch.float32, device=dev)
+    _ws, wp, wn = _workspace("tj_layernorm_backward_workspace_bytes", dev, rows, d)
+    _run(index, "tj_layernorm_backward", dy.data_ptr(), _DTYPES[dy.dtype], xp, xs, weight.data_ptr(), mean.data_ptr(),
+         rstd.data_ptr(), rows, d, mptr, rp, dx.data_ptr(), _DTYPES[x.dtype], dweight.data_ptr(), dbias.data_ptr(), wp,
+         wn)
     return dx, dweight, dbias
-
-
-_workspace_bytes: dict = {}
-
-
-def _workspace(name: str, device: torch.device, *sizes: int) -> torch.Tensor:
-    """A fresh workspace from torch's allocator (so that calls on different
-    streams, or captured into different graphs, never share one); only the
-    size that a shape needs is kept."""
-    key = (name, device.index, sizes)
-    n = _workspace_bytes.get(key)
-    if n is None:
-        nbytes = ctypes.c_size_t()
-        with torch.cuda.device(device):
-            _lib.call(name, *sizes, ctypes.byref(nbytes))
-        if len(_workspace_bytes) >= 4096:
-            _workspace_bytes.clear()
-        n = _workspace_bytes[key] = int(nbytes.value)
-    return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 def gelu_backward(dy: torch.Tensor, h, mask: Optional[torch.Tensor] = None, pack: bool = False):
     """dh = dy * gelu'(h) (exact GELU) for dy [rows, cols] (fp32, fp16 or
     bf16); h: the input of the GELU in dy's type, or its 8-bit copy.  ``pack``
     returns (dh, Act8 of dh) in one pass."""
-    _matrix(dy, "dy", _DTYPES)
-    rows, cols = dy.shape
+    index = _matrix(dy, "dy", _DTYPES)
+    rows, cols = shape = dy.shape
     if isinstance(h, Act8):
-        _check_act(h, "h", dy.device)
-        ht, hs = h.codes, h.scales.data_ptr()
+        if _check_act(h, "h", index)[1:] != shape:
+            raise ValueError(f"h: shape {tuple(h.codes.shape)}, need {tuple(shape)}")
+        hp, hs = h.codes.data_ptr(), h.scales.data_ptr()
     else:
-        _matrix(h, "h", (dy.dtype,), device=dy.device)
-        ht, hs = h, None
-    if ht.shape != dy.shape:
-        raise ValueError(f"h: shape {tuple(ht.shape)}, need {tuple(dy.shape)}")
-    mptr = _row_mask(mask, rows, dy.device)
+        _matrix(h, "h", (dy.dtype,), shape, index)
+        hp, hs = h.data_ptr(), None
+    mptr = _row_mask(mask, rows, index)
     dh = torch.empty_like(dy)
     dh8 = _new_act(rows, cols, dy.device, dy.dtype) if pack else None
-    _run(dy.device, "tj_gelu_backward", dy.data_ptr(), _DTYPES[dy.dtype], ht.data_ptr(), hs, rows, cols, mptr,
-         dh.data_ptr(), dh8.codes.data_ptr() if pack else None, dh8.scales.data_ptr() if pack else None)
+    _run(index, "tj_gelu_backward", dy.data_ptr(), _DTYPES[dy.dtype], hp, hs, rows, cols, mptr, dh.data_ptr(),
+         dh8.codes.data_ptr() if pack else None, dh8.scales.data_ptr() if pack else None)
     return (dh, dh8) if pack else dh
 
 
 def _check_product(a: Act8, w: Weight8, bias, what: str, step: int):
-    _check_act(a, "a")
+    index, m, k = _check_act(a, "a")
     if not isinstance(w, Weight8):
         raise ValueError("w must be a Weight8")
-    _check8(w, "w", lambda r, c: (_blocks(r), _blocks(c)), a.codes.device)
-    m, k = a.codes.shape
-    n = w.codes.shape[0]
-    if w.codes.shape[1] != k:
-        raise ValueError(f"w: shape {tuple(w.codes.shape)}, need [n, {k}]")
+    _matrix(w.codes, "w", (_E4M3,), None, index)
+    n, wk = w.codes.shape
+    if wk != k:
+        raise ValueError(f"w: shape {(n, wk)}, need [n, {k}]")
     if n == 0 or n % step or k % 16:
         raise ValueError(f"{what} needs n % {step} == 0 and k % 16 == 0, got n {n}, k {k}")
-    if bias is not None:
-        _matrix(bias, "bias", (torch.float32,), (n,), a.codes.device)
-    return m, n, k
+    _matrix(w.scales, "w", (_E8M0,), (_blocks(n), _blocks(k)), index)
+    if bias is None:
+        return index, m, n, k, None
+    _matrix(bias, "bias", _F32, (n,), index)
+    return index, m, n, k, bias.data_ptr()
 
 
 def gemm8(a: Act8, w: Weight8, bias: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
@@ -446,19 +473,20 @@ def gemm8(a: Act8, w: Weight8, bias: Optional[torch.Tensor] = None, mask: Option
     """a @ w.T [+ bias] [+ resid] on 8-bit operands with FP32 sums; ``resid``
     (fp32 [m, n]) needs out_dtype torch.float32.  n % 8 == 0, k % 16 == 0.
     ``err``: the error word to use instead of the device's own."""
-    m, n, k = _check_product(a, w, bias, "gemm8", 8)
+    index, m, n, k, bp = _check_product(a, w, bias, "gemm8", 8)
     if out_dtype not in _DTYPES:
         raise ValueError(f"out_dtype {out_dtype} not supported")
-    dev = a.codes.device
+    rp = None
     if resid is not None:
         if out_dtype != torch.float32:
             raise ValueError("resid needs out_dtype torch.float32")
-        _matrix(resid, "resid", (torch.float32,), (m, n), dev)
-    mptr = _row_mask(mask, m, dev)
-    err = _err_word(dev) if err is None else err
-    out = torch.empty(m, n, dtype=out_dtype, device=dev)
-    _run(dev, "tj_gemm8", a.codes.data_ptr(), a.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(),
-         _ptr(bias), m, n, k, mptr, _ptr(resid), out.data_ptr(), _DTYPES[out_dtype], err.data_ptr())
+        _matrix(resid, "resid", _F32, (m, n), index)
+        rp = resid.data_ptr()
+    mptr = _row_mask(mask, m, index)
+    ep = _err_ptr(err, index)
+    out = torch.empty(m, n, dtype=out_dtype, device=a.codes.device)
+    _run(index, "tj_gemm8", a.codes.data_ptr(), a.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), bp, m, n, k,
+         mptr, rp, out.data_ptr(), _DTYPES[out_dtype], ep)
     return out
 
 
@@ -467,14 +495,13 @@ def gemm8_gelu(a: Act8, w: Weight8, bias: Optional[torch.Tensor] = None, mask: O
     """(gelu(h), h) in 8 bits for h = a @ w.T [+ bias]: the FFN-in layer, whose
     output feeds the next product and whose h serves ``gelu_backward``.
     n % 16 == 0, k % 16 == 0."""
-    m, n, k = _check_product(a, w, bias, "gemm8_gelu", 16)
+    index, m, n, k, bp = _check_product(a, w, bias, "gemm8_gelu", 16)
     dev = a.codes.device
-    mptr = _row_mask(mask, m, dev)
-    err = _err_word(dev) if err is None else err
+    mptr = _row_mask(mask, m, index)
+    ep = _err_ptr(err, index)
     g, h = _new_act(m, n, dev, a.dtype), _new_act(m, n, dev, a.dtype)
-    _run(dev, "tj_gemm8_gelu", a.codes.data_ptr(), a.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(),
-         _ptr(bias), m, n, k, mptr, g.codes.data_ptr(), g.scales.data_ptr(), h.codes.data_ptr(), h.scales.data_ptr(),
-         err.data_ptr())
+    _run(index, "tj_gemm8_gelu", a.codes.data_ptr(), a.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), bp, m,
+         n, k, mptr, g.codes.data_ptr(), g.scales.data_ptr(), h.codes.data_ptr(), h.scales.data_ptr(), ep)
     return g, h
 
 
@@ -483,20 +510,20 @@ def linear_wgrad(dy: torch.Tensor, x: Act8, mask: Optional[torch.Tensor] = None,
     """Gradients (dweight [n, k], dbias [n], fp32) of a linear layer for dy
     [rows, n] (fp16 or bf16) and the 8-bit copy of its input [rows, k].  x
     enters the product in dy's type: exact in bf16, as ``restore8`` in fp16.
-    n % 8 == 0, k % 16 == 0."""
-    _matrix(dy, "dy", (torch.float16, torch.bfloat16))
-    _check_act(x, "x", dy.device)
+    n % 8 == 0, k % 16 == 0.  Takes a workspace of 2 * rows * k bytes and more."""
+    index = _matrix(dy, "dy", (torch.float16, torch.bfloat16))
     rows, n = dy.shape
-    if x.codes.shape[0] != rows:
-        raise ValueError(f"x: {x.codes.shape[0]} rows, need {rows}")
-    k = x.codes.shape[1]
+    _, xrows, k = _check_act(x, "x", index)
+    if xrows != rows:
+        raise ValueError(f"x: {xrows} rows, need {rows}")
     if n % 8 or k % 16:
         raise ValueError(f"linear_wgrad needs n % 8 == 0 and k % 16 == 0, got n {n}, k {k}")
-    mptr = _row_mask(mask, rows, dy.device)
-    err = _err_word(dy.device) if err is None else err
-    dw = torch.empty(n, k, dtype=torch.float32, device=dy.device)
-    db = torch.empty(n, dtype=torch.float32, device=dy.device)
-    ws = _workspace("tj_wgrad8_workspace_bytes", dy.device, rows, n, k)
-    _run(dy.device, "tj_wgrad8", dy.data_ptr(), _DTYPES[dy.dtype], x.codes.data_ptr(), x.scales.data_ptr(), rows, n, k,
-         mptr, dw.data_ptr(), db.data_ptr(), ws.data_ptr(), ws.numel(), err.data_ptr())
+    mptr = _row_mask(mask, rows, index)
+    ep = _err_ptr(err, index)
+    dev = dy.device
+    dw = torch.empty(n, k, dtype=torch.float32, device=dev)
+    db = torch.empty(n, dtype=torch.float32, device=dev)
+    _ws, wp, wn = _workspace("tj_wgrad8_workspace_bytes", dev, rows, n, k)
+    _run(index, "tj_wgrad8", dy.data_ptr(), _DTYPES[dy.dtype], x.codes.data_ptr(), x.scales.data_ptr(), rows, n, k, mptr,
+         dw.data_ptr(), db.data_ptr(), wp, wn, ep)
     return dw, db
