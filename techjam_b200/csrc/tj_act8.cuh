@@ -263,10 +263,8 @@ __global__ void __launch_bounds__(256) act8_pack_kernel(const T* __restrict__ x,
 }
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) act8_unpack_kernel(const uint8_t* __restrict__ codes,
-                                                          const uint8_t* __restrict__ scales, long long rows,
-                                                          int cols, const uint8_t* __restrict__ mask,
-                                                          T* __restrict__ out) {
+TJ_DEV void act8_unpack(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, long long rows, int cols,
+                        const uint8_t* __restrict__ mask, T* __restrict__ out) {
   const BlockAt b = block_at(rows, cols);
   const int sub = threadIdx.x & 7;
   if (!b.live) return;
@@ -285,6 +283,12 @@ __global__ void __launch_bounds__(256) act8_unpack_kernel(const uint8_t* __restr
     for (int i = 0; i < 4; ++i) o[i] = from_f32_restored<T>(v[i]);
     store4<T, VEC>(out + b.row * cols, b.c0, sub, j, cols, o);
   }
+}
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) act8_unpack_kernel(const uint8_t* __restrict__ codes,
+                                                          const uint8_t* __restrict__ scales, long long rows,
+                                                          int cols, T* __restrict__ out) {
+  act8_unpack<T, VEC>(codes, scales, rows, cols, nullptr, out);
 }
 
 // One CTA per 128 x 128 block of a weight [n, k]: codes [n, k] (or [k, n]
@@ -414,12 +418,11 @@ __global__ void __launch_bounds__(256) gelu_bwd_kernel(const T* __restrict__ dy,
 // has 8 columns (a 32-byte sector of a row), its 128 groups of 8 lanes every
 // 128th row each; joined in a fixed order.  (32 columns to a CTA: 7.6 us for
 // 592 x 2048, too few CTAs.)
-static __global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restrict__ in, int n, int cols,
-                                                                 float* __restrict__ out0, float* __restrict__ out1,
-                                                                 int split) {
+TJ_DEV void column_sum(const float* __restrict__ in, int n, int cols, float* __restrict__ out0,
+                       float* __restrict__ out1, int split, unsigned block) {
   __shared__ float s[128][9];
   const int col = threadIdx.x & 7, grp = threadIdx.x >> 3;
-  const int c = blockIdx.x * 8 + col;
+  const int c = block * 8 + col;
   float a = 0.f;
   if (c < cols) {
     for (int r0 = grp; r0 < n; r0 += 128 * 8) {
@@ -435,12 +438,18 @@ static __global__ void __launch_bounds__(1024) column_sum_kernel(const float* __
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (w < 8) {
     const float t = warp_sum((s[lane][w] + s[lane + 32][w]) + (s[lane + 64][w] + s[lane + 96][w]));
-    const int cc = blockIdx.x * 8 + w;
+    const int cc = block * 8 + w;
     if (lane == 0 && cc < cols) {
       if (cc < split) out0[cc] = t;
       else out1[cc - split] = t;
     }
   }
+}
+
+static __global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restrict__ in, int n, int cols,
+                                                                 float* __restrict__ out0, float* __restrict__ out1,
+                                                                 int split) {
+  column_sum(in, n, cols, out0, out1, split, blockIdx.x);
 }
 
 }  // namespace tj

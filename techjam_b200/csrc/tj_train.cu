@@ -43,10 +43,10 @@ int pack_t(const void* x, long long rows, int cols, const uint8_t* mask, uint8_t
   return TJ_OK;
 }
 template <typename T>
-int unpack_t(const uint8_t* codes, const uint8_t* scales, long long rows, int cols, const uint8_t* mask, void* out,
-             bool vec, unsigned grid, cudaStream_t st) {
-  if (vec) tj::act8_unpack_kernel<T, true><<<grid, 256, 0, st>>>(codes, scales, rows, cols, mask, static_cast<T*>(out));
-  else tj::act8_unpack_kernel<T, false><<<grid, 256, 0, st>>>(codes, scales, rows, cols, mask, static_cast<T*>(out));
+int unpack_t(const uint8_t* codes, const uint8_t* scales, long long rows, int cols, void* out, bool vec,
+             unsigned grid, cudaStream_t st) {
+  if (vec) tj::act8_unpack_kernel<T, true><<<grid, 256, 0, st>>>(codes, scales, rows, cols, static_cast<T*>(out));
+  else tj::act8_unpack_kernel<T, false><<<grid, 256, 0, st>>>(codes, scales, rows, cols, static_cast<T*>(out));
   TJH_CUDA(cudaGetLastError());
   return TJ_OK;
 }
@@ -283,9 +283,9 @@ int tj_act8_unpack(const void* codes, const uint8_t* scales, long long rows, int
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const uint8_t* c = static_cast<const uint8_t*>(codes);
   switch (dtype) {
-    case TJ_F32: return unpack_t<float>(c, scales, rows, cols, nullptr, out, vec, grid, st);
-    case TJ_F16: return unpack_t<__half>(c, scales, rows, cols, nullptr, out, vec, grid, st);
-    default: return unpack_t<__nv_bfloat16>(c, scales, rows, cols, nullptr, out, vec, grid, st);
+    case TJ_F32: return unpack_t<float>(c, scales, rows, cols, out, vec, grid, st);
+    case TJ_F16: return unpack_t<__half>(c, scales, rows, cols, out, vec, grid, st);
+    default: return unpack_t<__nv_bfloat16>(c, scales, rows, cols, out, vec, grid, st);
   }
 }
 
@@ -404,29 +404,30 @@ int tj_wgrad8(const void* dy, int dtype, const void* x8_codes, const uint8_t* x8
   p.dw = w.splits > 1 ? reinterpret_cast<float*>(base + w.dw) : dw;
   p.db = reinterpret_cast<float*>(base + w.db);
   p.err = err;
-  if (mask != nullptr) {
-    int* list = reinterpret_cast<int*>(base + w.list);
-    tj::wgrad8_list_kernel<<<1, 1024, 0, st>>>(mask, rows, list + 1, list);
-    TJH_CUDA(cudaGetLastError());
+  int* list = mask != nullptr ? reinterpret_cast<int*>(base + w.list) : nullptr;
+  if (list != nullptr) {
     p.list = list + 1;
     p.n_list = list;
   }
   unsigned grid;
   TJH_CHECK(block_grid(rows, k, &grid));
+  const unsigned blocks = grid + (list != nullptr ? 1u : 0u);
   const uint8_t* codes = static_cast<const uint8_t*>(x8_codes);
   if (dtype == TJ_F16) {
-    TJH_CHECK(unpack_t<__half>(codes, x8_scales, rows, k, mask, base + w.x, true, grid, st));
+    tj::wgrad8_prep_kernel<__half><<<blocks, 256, 0, st>>>(codes, x8_scales, rows, k, mask, reinterpret_cast<__half*>(base + w.x),
+                                                           grid, list ? list + 1 : nullptr, list);
+    TJH_CUDA(cudaGetLastError());
     TJH_CHECK(launch_wgrad8<__half>(dy, base + w.x, p, dev, sms, st));
   } else {
-    TJH_CHECK(unpack_t<__nv_bfloat16>(codes, x8_scales, rows, k, mask, base + w.x, true, grid, st));
+    tj::wgrad8_prep_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(
+        codes, x8_scales, rows, k, mask, reinterpret_cast<__nv_bfloat16*>(base + w.x), grid, list ? list + 1 : nullptr, list);
+    TJH_CUDA(cudaGetLastError());
     TJH_CHECK(launch_wgrad8<__nv_bfloat16>(dy, base + w.x, p, dev, sms, st));
   }
-  if (w.splits > 1) {
-    const long long total = (long long)n * k;
-    tj::wgrad8_join_kernel<<<(unsigned)((total / 4 + 255) / 256), 256, 0, st>>>(p.dw, w.splits, total, dw);
-    TJH_CUDA(cudaGetLastError());
-  }
-  tj::column_sum_kernel<<<(n + 7) / 8, 1024, 0, st>>>(p.db, 4 * w.splits * w.k_tiles, n, db, db, n);
+  const long long total = (long long)n * k;
+  const unsigned join = w.splits > 1 ? (unsigned)((total / 4 + 1023) / 1024) : 0u;
+  tj::wgrad8_finish_kernel<<<join + (n + 7) / 8, 1024, 0, st>>>(p.dw, w.splits, total, dw, join, p.db,
+                                                                4 * w.splits * w.k_tiles, n, db);
   TJH_CUDA(cudaGetLastError());
   return TJ_OK;
 }

@@ -60,17 +60,15 @@ struct Wgrad8Params {
   int* err;
 };
 
-// Stages of 64 tokens that hold a valid one, in order.  One block.
-__global__ void __launch_bounds__(1024) wgrad8_list_kernel(const uint8_t* __restrict__ mask, long long T,
-                                                           int* __restrict__ list, int* __restrict__ n_list) {
-  __shared__ int s_warp[32];
-  __shared__ int s_base;
+// Stages of 64 tokens that hold a valid one, in order (256 threads).
+TJ_DEV void wgrad8_list(const uint8_t* __restrict__ mask, long long T, int* __restrict__ list,
+                        int* __restrict__ n_list) {
+  __shared__ int s_warp[8];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  if (threadIdx.x == 0) s_base = 0;
-  __syncthreads();
   const int stages = (int)((T + kWgTok - 1) / kWgTok);
-  for (int s0 = 0; s0 < stages; s0 += blockDim.x) {
-    const int s = s0 + threadIdx.x;
+  int before = 0;
+  for (int s0 = 0; s0 < stages; s0 += 256) {
+    const int s = s0 + (int)threadIdx.x;
     int n = 0, full = 0;
     if (s < stages) {
       const long long t0 = (long long)s * kWgTok;
@@ -84,41 +82,56 @@ __global__ void __launch_bounds__(1024) wgrad8_list_kernel(const uint8_t* __rest
                 __popc(__vcmpne4(v.w, 0u))) >> 3;
         }
       } else {
+#pragma unroll 8
         for (int i = 0; i < full; ++i) n += mask[t0 + i] != 0;
       }
     }
     const int live = n > 0 ? 1 : 0;
-    int incl = live;
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += u;
-    }
-    if (lane == 31) s_warp[w] = incl;
+    const uint32_t vote = __ballot_sync(0xffffffffu, live);
+    if (lane == 0) s_warp[w] = __popc(vote);
     __syncthreads();
-    if (w == 0) {
-      int v = s_warp[lane];
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += u;
-      }
-      s_warp[lane] = v;
+    int at = before + __popc(vote & ((1u << lane) - 1u));
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int c = s_warp[q];
+      if (q < w) at += c;
+      before += c;
     }
-    __syncthreads();
-    const int at = s_base + incl - live + (w > 0 ? s_warp[w - 1] : 0);
     if (live) list[at] = s | (n < full ? (int)0x80000000 : 0);
     __syncthreads();
-    if (threadIdx.x == blockDim.x - 1) s_base = at + live;
-    __syncthreads();
   }
-  if (threadIdx.x == 0) *n_list = s_base;
+  if (threadIdx.x == 0) *n_list = before;
 }
 
-// out[i] = sum over s of in[s][i] for i < n (n a multiple of 4), in order.
-__global__ void __launch_bounds__(256) wgrad8_join_kernel(const float* __restrict__ in, int splits, long long n,
-                                                          float* __restrict__ out) {
+// Before the product: X restored to T (zeros in masked rows), and in one block
+// more the stage list.  One launch for both: a launch is 3 us of a small call.
+template <typename T>
+__global__ void __launch_bounds__(256) wgrad8_prep_kernel(const uint8_t* __restrict__ codes,
+                                                          const uint8_t* __restrict__ scales, long long rows, int cols,
+                                                          const uint8_t* __restrict__ mask, T* __restrict__ out,
+                                                          unsigned unpack_blocks, int* __restrict__ list,
+                                                          int* __restrict__ n_list) {
+  if (blockIdx.x == unpack_blocks) {
+    wgrad8_list(mask, rows, list, n_list);
+    return;
+  }
+  act8_unpack<T, true>(codes, scales, rows, cols, mask, out);
+}
+
+// After it: the first blocks add up the parts of dW (n values, a multiple of
+// 4; out[i] = sum over s of in[s][i], in order), the others db's columns.
+__global__ void __launch_bounds__(1024) wgrad8_finish_kernel(const float* __restrict__ in, int splits, long long n,
+                                                             float* __restrict__ out, unsigned join_blocks,
+                                                             const float* __restrict__ db_in, int db_rows, int db_n,
+                                                             float* __restrict__ db) {
+  if (blockIdx.x >= join_blocks) {
+    column_sum(db_in, db_rows, db_n, db, db, db_n, blockIdx.x - join_blocks);
+    return;
+  }
   const long long i = 4 * ((long long)blockIdx.x * blockDim.x + threadIdx.x);
   if (i >= n) return;
   float4 a = *reinterpret_cast<const float4*>(in + i);
+#pragma unroll 4
   for (int s = 1; s < splits; ++s) {
     const float4 b = *reinterpret_cast<const float4*>(in + (long long)s * n + i);
     a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
@@ -272,18 +285,24 @@ __global__ void __launch_bounds__(kWgThreads, 1)
         for (int s = im.s0; s < im.s1; ++s) {
           const int entry = p.list[s];
           if (entry < 0) {
+            // the mask before the wait: the tile is then cleared as it lands,
+            // stages before its MMAs
+            const long long t0 = (long long)(entry & 0x7fffffff) * kWgTok;
+            uint32_t out[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const long long t = t0 + 32 * h + lane;
+              out[h] = __ballot_sync(0xffffffffu, t < p.T && __ldg(p.mask + t) == 0);
+            }
             if (!mbar_wait_warp(a_full + stage, (abits >> stage) & 1u, p.err, kErrWgradEdge)) { ok = false; break; }
             abits ^= 1u << stage;
             uint8_t* sa = smem + stage * kWgStageBytes;
-            const long long t0 = (long long)(entry & 0x7fffffff) * kWgTok;
-            for (int h = 0; h < 2; ++h) {
-              const long long t = t0 + 32 * h + lane;
-              uint32_t out = __ballot_sync(0xffffffffu, t < p.T && __ldg(p.mask + t) == 0);
-              for (; out != 0; out &= out - 1) {  // 16 lanes clear a token's 256 bytes
-                const int tok = 32 * h + __ffs(out) - 1;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              for (uint32_t left = out[h]; left != 0; left &= left - 1) {  // 16 lanes clear a token's 256 bytes
+                const int tok = 32 * h + __ffs(left) - 1;
                 if (lane < 16) *reinterpret_cast<uint4*>(sa + (lane >> 3) * 8192 + tok * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
               }
-            }
             fence_async_smem();
             __syncwarp();
             mbar_arrive_cluster_release(cleared0 + (uint32_t)(stage * sizeof(uint64_t)));
