@@ -196,11 +196,10 @@ TJ_DEV uint64_t gelu8_x2(uint64_t x) {
   const float2 tail = f32x2_split(fmul_x2(fmul_x2(t, q), f32x2(fast_exp2(-yy.x), fast_exp2(-yy.y))));
   return f32x2(fmaf(-fabsf(v.x), tail.x, fmaxf(v.x, 0.f)), fmaf(-fabsf(v.y), tail.y, fmaxf(v.y, 0.f)));
 }
-TJ_DEV uint32_t e4m3_pair(uint64_t x, uint64_t inv) {  // no infinities
-  uint16_t r;
-  const float2 v = f32x2_split(fmul_x2(x, inv));
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(v.y), "f"(v.x));
-  return r;
+// Codes of four values that are no infinities, times inv (twice the same).
+TJ_DEV uint32_t e4m3_pairs(uint64_t x, uint64_t y, uint64_t inv) {
+  const float2 a = f32x2_split(fmul_x2(x, inv)), b = f32x2_split(fmul_x2(y, inv));
+  return e4m3_word(a.x, a.y, b.x, b.y);
 }
 
 // GELU epilogue of N columns (a block of 128, or half of one) of one row: h in
@@ -255,13 +254,18 @@ TJ_DEV void gelu_pack_row(uint64_t (&h)[N / 2], bool valid, uint8_t* bufg, uint8
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint64_t v0 = h[8 * j + 2 * i], v1 = h[8 * j + 2 * i + 1];
-      gw[i] = __byte_perm(e4m3_pair(gelu8_x2(v0), ginv), e4m3_pair(gelu8_x2(v1), ginv), 0x5410);
-      hw[i] = __byte_perm(e4m3_pair(v0, hinv), e4m3_pair(v1, hinv), 0x5410);
+      gw[i] = e4m3_pairs(gelu8_x2(v0), gelu8_x2(v1), ginv);
+      hw[i] = e4m3_pairs(v0, v1, hinv);
     }
-    *reinterpret_cast<uint4*>(staged(bufg, lane, piece0 + j)) =
-        valid ? make_uint4(gw[0], gw[1], gw[2], gw[3]) : make_uint4(0, 0, 0, 0);
-    *reinterpret_cast<uint4*>(staged(bufh, lane, piece0 + j)) =
-        valid ? make_uint4(hw[0], hw[1], hw[2], hw[3]) : make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(staged(bufg, lane, piece0 + j)) = make_uint4(gw[0], gw[1], gw[2], gw[3]);
+    *reinterpret_cast<uint4*>(staged(bufh, lane, piece0 + j)) = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+  }
+  if (!valid) {
+#pragma unroll
+    for (int j = 0; j < N / 16; ++j) {
+      *reinterpret_cast<uint4*>(staged(bufg, lane, piece0 + j)) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(staged(bufh, lane, piece0 + j)) = make_uint4(0, 0, 0, 0);
+    }
   }
 }
 // h = the bias of columns col0.. (zeros past n), and h += 32 accumulator columns.
@@ -659,7 +663,7 @@ struct Gemm8PairCfg {
   static constexpr int kSfSlots = 2;
   static constexpr int kSfCols = 12;  // 4 for A's 128 rows, 8 for W's 256
   static constexpr int kThreads = 256 + 32 * kEpiWarps;
-  static constexpr int kRegLaunch = KIND == kG8Gelu ? 80 : 128;  // kG8Gelu: warpgroups with 40 + 56 + 4 * 96
+  static constexpr int kRegLaunch = KIND == kG8Gelu ? 80 : 128;  // kG8Gelu: warpgroups with 24 + 40 + 4 * 104 (96: 55 us for 47)
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kStagingBytes + 256;
   static_assert(kSmemBytes <= 232448, "shared memory");
 };
@@ -727,7 +731,7 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
   };
 
   if (warp < 4) {
-    if constexpr (KIND == kG8Gelu) reg_dealloc<40>();
+    if constexpr (KIND == kG8Gelu) reg_dealloc<24>();
     if (warp == 0) {
       // ---------------------------------------------------------- TMA producer
       if (lane == 0) { tma_prefetch_desc(&tmA); tma_prefetch_desc(&tmW); }
@@ -801,7 +805,7 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
     }
   } else if (warp < 8) {
     // ------------------------------------------------------------ scales -> TMEM
-    if constexpr (KIND == kG8Gelu) reg_dealloc<56>();
+    if constexpr (KIND == kG8Gelu) reg_dealloc<40>();
     // The words of a group of four K blocks are on their way a group ahead,
     // across tiles, so that no slot waits for global memory.
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -851,7 +855,7 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
     }
   } else {
     // ------------------------------------------------------------ epilogue
-    if constexpr (KIND == kG8Gelu) reg_alloc<96>();
+    if constexpr (KIND == kG8Gelu) reg_alloc<104>();
     const int ew = warp - 8, quarter = warp & 3;
     constexpr int kGroups = Cfg::kEpiWarps / 4, kCW = 256 / kGroups;
     const int cg = ew >> 2;  // column group
