@@ -274,16 +274,20 @@ __global__ void __launch_bounds__(256) act8_pack_kernel(const T* __restrict__ x,
   pack_block<VEC>(v, b.c0, cols, codes + b.row * cols, scales + b.row * n_blocks(cols) + b.blk, sub, b.live);
 }
 
+// (Pieces of 8 or 16 codes a lane, for wider stores, and two or four blocks a
+// lane measured the same or slower, 20-23 us for 33.5M codes to bf16: two
+// thirds of the traffic are writes.)
 template <typename T, bool VEC>
 TJ_DEV void act8_unpack(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, long long rows, int cols,
-                        T* __restrict__ out) {
+                        const uint8_t* __restrict__ mask, T* __restrict__ out) {
   const BlockAt b = block_at(rows, cols);
   const int sub = threadIdx.x & 7;
   if (!b.live) return;
-  const float s = scale_value(scales[b.row * n_blocks(cols) + b.blk]);
+  const bool valid = mask == nullptr || mask[b.row] != 0;
+  const float s = valid ? scale_value(scales[b.row * n_blocks(cols) + b.blk]) : 0.f;
   uint32_t w[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) w[j] = load_codes4<VEC>(codes + b.row * cols, b.c0, sub, j, cols);
+  for (int j = 0; j < 4; ++j) w[j] = load_codes4<VEC>(codes + b.row * cols, b.c0, sub, j, valid ? cols : 0);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     float v[4];
@@ -294,46 +298,11 @@ TJ_DEV void act8_unpack(const uint8_t* __restrict__ codes, const uint8_t* __rest
     store4<T, VEC>(out + b.row * cols, b.c0, sub, j, cols, o);
   }
 }
-// The same to 16 bits with 8 neighbouring codes a lane and piece (widths a
-// multiple of 8, rows aligned): 16-byte stores side by side.  (16 codes a lane
-// left 32 bytes between a store's lanes: 23 us for 33.5M codes to bf16, against
-// 21 with 4 a lane.)
-template <typename T>
-TJ_DEV void act8_unpack8(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, long long rows,
-                         int cols, const uint8_t* __restrict__ mask, T* __restrict__ out) {
-  static_assert(sizeof(T) == 2, "16-bit types");
-  const BlockAt b = block_at(rows, cols);
-  if (!b.live) return;
-  const bool valid = mask == nullptr || mask[b.row] != 0;
-  const int c0 = b.c0 + 8 * (threadIdx.x & 7);
-  uint2 w[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-    w[j] = valid && c0 + 64 * j < cols ? *reinterpret_cast<const uint2*>(codes + b.row * cols + c0 + 64 * j)
-                                       : make_uint2(0, 0);
-  const uint32_t byte = valid ? scales[b.row * n_blocks(cols) + b.blk] : 127u;
-  const float s = scale_value(byte);
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    alignas(16) T o[8];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float v[4];
-      e4m3x4_value(h == 0 ? w[j].x : w[j].y, s, v);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[4 * h + i] = byte < 135u ? from_f32<T>(v[i]) : from_f32_restored<T>(v[i]);
-    }
-    if (c0 + 64 * j < cols)
-      *reinterpret_cast<uint4*>(out + b.row * cols + c0 + 64 * j) = *reinterpret_cast<const uint4*>(o);
-  }
-}
-// MODE 0: element by element, 1: 4 codes at a time, 2: 8 (16-bit types).
-template <typename T, int MODE>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) act8_unpack_kernel(const uint8_t* __restrict__ codes,
                                                           const uint8_t* __restrict__ scales, long long rows,
                                                           int cols, T* __restrict__ out) {
-  if constexpr (MODE == 2) act8_unpack8<T>(codes, scales, rows, cols, nullptr, out);
-  else act8_unpack<T, MODE == 1>(codes, scales, rows, cols, out);
+  act8_unpack<T, VEC>(codes, scales, rows, cols, nullptr, out);
 }
 
 // One CTA per 128 x 128 block of a weight [n, k]: codes [n, k] (or [k, n]

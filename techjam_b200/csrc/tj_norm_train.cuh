@@ -72,9 +72,16 @@ struct NormFwdParams {
   float eps;
 };
 
+// CTAs per SM forward.  What hides the loads is rows in flight: 32768 x 1024
+// fp32 to fp16, padded, took 41, 35 and 32 us with 4, 6 and 8; packing and the
+// scalar loads need the registers of 6 (48 us to 8 bits with a copy of x, 49
+// with 8).
+template <typename Y>
+constexpr int norm_fwd_ctas(bool vec) { return std::is_same_v<Y, uint8_t> || !vec ? 6 : 8; }
+
 // NI: 512-column steps per warp (1 or 2).
 template <typename T, typename Y, int WR, int NI, bool VEC>
-__global__ void __launch_bounds__(32 * kNormWarps, 6) norm_fwd_kernel(const NormFwdParams p) {
+__global__ void __launch_bounds__(32 * kNormWarps, norm_fwd_ctas<Y>(VEC)) norm_fwd_kernel(const NormFwdParams p) {
   __shared__ float s_red[2][kNormWarps];
   int red = 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

@@ -43,14 +43,10 @@ int pack_t(const void* x, long long rows, int cols, const uint8_t* mask, uint8_t
   return TJ_OK;
 }
 template <typename T>
-int unpack_t(const uint8_t* codes, const uint8_t* scales, long long rows, int cols, void* out, int mode,
+int unpack_t(const uint8_t* codes, const uint8_t* scales, long long rows, int cols, void* out, bool vec,
              unsigned grid, cudaStream_t st) {
-  T* o = static_cast<T*>(out);
-  if constexpr (sizeof(T) == 2) {
-    if (mode == 2) tj::act8_unpack_kernel<T, 2><<<grid, 256, 0, st>>>(codes, scales, rows, cols, o);
-  }
-  if (mode == 1) tj::act8_unpack_kernel<T, 1><<<grid, 256, 0, st>>>(codes, scales, rows, cols, o);
-  if (mode == 0) tj::act8_unpack_kernel<T, 0><<<grid, 256, 0, st>>>(codes, scales, rows, cols, o);
+  if (vec) tj::act8_unpack_kernel<T, true><<<grid, 256, 0, st>>>(codes, scales, rows, cols, static_cast<T*>(out));
+  else tj::act8_unpack_kernel<T, false><<<grid, 256, 0, st>>>(codes, scales, rows, cols, static_cast<T*>(out));
   TJH_CUDA(cudaGetLastError());
   return TJ_OK;
 }
@@ -284,15 +280,13 @@ int tj_act8_unpack(const void* codes, const uint8_t* scales, long long rows, int
   if (!plain(dtype)) return fail(TJ_ERR_INVALID, "unknown dtype %d", dtype);
   if (rows == 0) return TJ_OK;
   if (!out || !codes || !scales) return fail(TJ_ERR_INVALID, "null argument");
-  const bool vec8 = dtype != TJ_F32 && cols % 8 == 0 && aligned(out, 16) && aligned(codes, 8);
-  const bool vec4 = cols % 4 == 0 && aligned(out, vec_bytes(dtype)) && aligned(codes, 4);
-  const int mode = vec8 ? 2 : (vec4 ? 1 : 0);
+  const bool vec = cols % 4 == 0 && aligned(out, vec_bytes(dtype)) && aligned(codes, 4);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const uint8_t* c = static_cast<const uint8_t*>(codes);
   switch (dtype) {
-    case TJ_F32: return unpack_t<float>(c, scales, rows, cols, out, mode, grid, st);
-    case TJ_F16: return unpack_t<__half>(c, scales, rows, cols, out, mode, grid, st);
-    default: return unpack_t<__nv_bfloat16>(c, scales, rows, cols, out, mode, grid, st);
+    case TJ_F32: return unpack_t<float>(c, scales, rows, cols, out, vec, grid, st);
+    case TJ_F16: return unpack_t<__half>(c, scales, rows, cols, out, vec, grid, st);
+    default: return unpack_t<__nv_bfloat16>(c, scales, rows, cols, out, vec, grid, st);
   }
 }
 

@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(256) wgrad8_prep_kernel(const uint8_t* __restr
     wgrad8_list(mask, rows, list, n_list);
     return;
   }
-  act8_unpack8<T>(codes, scales, rows, cols, mask, out);
+  act8_unpack<T, true>(codes, scales, rows, cols, mask, out);
 }
 
 // After it: the first blocks add up the parts of dW (n values, a multiple of
