@@ -176,21 +176,24 @@ TJ_DEV uint32_t pack_bf162(float a, float b) {
 // 128-byte TMA swizzle; conflict-free for one piece per lane).
 TJ_DEV uint8_t* staged(uint8_t* buf, int lane, int j) { return buf + lane * 128 + ((j ^ (lane & 7)) << 4); }
 
-// gelu(x) = max(x, 0) - |x| erfc(|x| / sqrt 2) / 2 for two values, erfc from
-// Abramowitz & Stegun 7.1.26 as in gelu_erf_x2 (nothing cancels for x < 0).
-// The SFU bounds this epilogue (8 cycles an operation and warp), so both
-// reciprocals come from that of the product: 1 / d0 = d1 / (d0 d1).
+// gelu(x) = max(x, 0) - |x| T(|x|) exp(-x^2 / 2) for two values, where
+// T(a) = erfc(a / sqrt 2) exp(a^2 / 2) / 2 is a polynomial in t = 1 / (1 + 0.225 a):
+// fitted here (iterated weighted least squares over 0 <= a <= 9) to 3e-9 in
+// T exp(-a^2 / 2) and 1.1e-7 relative.  (The five terms of gelu_erf_x2, 7.5e-8
+// off, moved more codes over a boundary than the 32-bit sums do.)  Nothing
+// cancels for x < 0.  Both reciprocals come from that of the product,
+// 1 / d0 = d1 / (d0 d1): the SFU takes 8 cycles an operation and warp.
 TJ_DEV uint64_t gelu8_x2(uint64_t x) {
-  constexpr float kP = 0.3275911f * 0.70710678118654752f;
   const float2 v = f32x2_split(x);
-  const float d0 = fmaf(fabsf(v.x), kP, 1.f), d1 = fmaf(fabsf(v.y), kP, 1.f);
+  const float d0 = fmaf(fabsf(v.x), 0.225f, 1.f), d1 = fmaf(fabsf(v.y), 0.225f, 1.f);
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d0 * d1));
   const uint64_t t = f32x2(r * d1, r * d0);
-  uint64_t q = ffma_x2(t, f32x2(0.5f * 1.061405429f, 0.5f * 1.061405429f), f32x2(-0.5f * 1.453152027f, -0.5f * 1.453152027f));
-  q = ffma_x2(t, q, f32x2(0.5f * 1.421413741f, 0.5f * 1.421413741f));
-  q = ffma_x2(t, q, f32x2(-0.5f * 0.284496736f, -0.5f * 0.284496736f));
-  q = ffma_x2(t, q, f32x2(0.5f * 0.254829592f, 0.5f * 0.254829592f));
+  constexpr float kC[8] = {0.09031444994160742f, 0.08178340952580349f, 0.1346013969305005f, -0.09456394526861704f,
+                           0.4214357682285032f, -0.4126644252272553f, 0.37029267947368516f, -0.09119933652481564f};
+  uint64_t q = f32x2(kC[7], kC[7]);
+#pragma unroll
+  for (int i = 6; i >= 0; --i) q = ffma_x2(t, q, f32x2(kC[i], kC[i]));
   const uint64_t y = fmul_x2(x, f32x2(0.84932180028801904f, 0.84932180028801904f));  // sqrt(log2(e) / 2)
   const float2 yy = f32x2_split(fmul_x2(y, y));
   const float2 tail = f32x2_split(fmul_x2(fmul_x2(t, q), f32x2(fast_exp2(-yy.x), fast_exp2(-yy.y))));
@@ -699,6 +702,8 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
   uint64_t* sf_full = shared_free + 1;    // [SF] (even CTA's copy)
   uint64_t* sf_empty = sf_full + SF;      // [SF]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sf_empty + SF);
+  volatile uint8_t* agreed = reinterpret_cast<volatile uint8_t*>(tmem_slot + 1);  // kG8Gelu: [2][16], an epilogue warp's wait succeeded
+  static_assert((2 * S + 5 + 2 * SF) * 8 + 4 + 32 <= 256, "barrier space");
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -863,6 +868,7 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
     uint8_t* bufs = staging + (KIND == kG8Gelu ? 4 * (cg >> 1) + quarter : ew) * 8192;
     const uint32_t acc_empty0 = map_to_rank(acc_empty, 0), shared_free0 = map_to_rank(shared_free, 0);
     uint32_t used = 0;  // staging buffers used so far
+    int turn = 0;       // kG8Gelu: set of flags of this tile
     int abuf = 0;
     uint32_t aphase = 0;
     bool ok = true;
@@ -909,13 +915,20 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
             free_acc();
             if (swap) add_pairs(h, r); else add_pairs(h + 16, r);
           }
-          if (!ok) break;
         }
         // the two warps of a block meet at a barrier of their own, and
-        // exchange their maxima in the staging before the codes fill it
+        // exchange their maxima in the staging before the codes fill it.
+        // Neither leaves alone, which would keep the other waiting for good:
+        // they agree first that both their waits succeeded.
         float2* other = reinterpret_cast<float2*>(bufs);
         const int bar_id = 1 + (cg >> 1) * 4 + quarter;
         auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(bar_id) : "memory"); };
+        volatile uint8_t* flags = agreed + 16 * turn;
+        turn ^= 1;
+        if (lane == 0) flags[ew] = ok ? 1 : 0;
+        meet();
+        ok = flags[ew] != 0 && flags[ew ^ 4] != 0;
+        if (!ok) break;
         const int cb = nt * 256 + (cg >> 1) * 128;  // the block's first column
         if (row0 < p.M && cb < p.N) {
           uint32_t gbyte, hbyte;

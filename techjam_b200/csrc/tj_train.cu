@@ -185,6 +185,7 @@ int launch_gemm8_pair(const Gemm8Args& g, const tj::Gemm8Params& p, int dev, cud
 int gemm8_params(tj::Gemm8Params* p, const void* a, const uint8_t* as, const void* w, const uint8_t* ws,
                  const float* bias, int m, int n, int k, const uint8_t* mask, int* err) {
   if (m < 0 || n <= 0 || k <= 0) return fail(TJ_ERR_INVALID, "product of [%d, %d] and [%d, %d]", m, k, n, k);
+  if (m > 0x7fffff00 || n > 0x7fffff00 || k > 0x7fffff00) return fail(TJ_ERR_UNSUPPORTED, "product too large");
   if (!w || !ws || !err || (m > 0 && (!a || !as))) return fail(TJ_ERR_INVALID, "null argument");
   if (k % 16) return fail(TJ_ERR_UNSUPPORTED, "need k %% 16 == 0");
   if (bias != nullptr && !aligned(bias, 16)) return fail(TJ_ERR_INVALID, "bias not 16-byte aligned");

@@ -179,6 +179,7 @@ def poly_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, exact_pref
 
 _DTYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 _F32 = (torch.float32,)
+_MAX = 0x7fffff00  # sizes that the entries take as int
 
 
 class Act8(NamedTuple):
@@ -226,7 +227,7 @@ def _matrix(t: torch.Tensor, what: str, dtypes, shape=None, index: Optional[int]
     """Check an operand ([rows, cols], or the given shape) and return its CUDA device's index."""
     at = t.get_device()
     if (at >= 0 and t.is_contiguous() and t.dtype in dtypes and (index is None or at == index)
-            and (t.shape == shape if shape is not None else t.dim() == 2 and t.shape[1] > 0)):
+            and (t.shape == shape if shape is not None else t.dim() == 2 and 0 < t.shape[1] < _MAX)):
         return at
     if at < 0 or not t.is_contiguous():
         raise ValueError(f"{what}: techjam_b200.ops needs contiguous CUDA tensors")
@@ -234,8 +235,8 @@ def _matrix(t: torch.Tensor, what: str, dtypes, shape=None, index: Optional[int]
         raise ValueError(f"{what}: dtype {t.dtype}, need one of {', '.join(map(str, dtypes))}")
     if index is not None and at != index:
         raise ValueError(f"{what}: on {t.device}, need cuda:{index}")
-    if t.dim() == 2 and t.shape[1] == 0:
-        raise ValueError(f"{what}: no columns")
+    if t.dim() == 2 and shape is None:
+        raise ValueError(f"{what}: {t.shape[1]} columns")
     raise ValueError(f"{what}: shape {tuple(t.shape)}, need {'[rows, cols]' if shape is None else tuple(shape)}")
 
 
@@ -333,8 +334,8 @@ def pack_weight8(w: torch.Tensor, transpose: bool = False) -> Weight8:
     the product that takes a gradient back through the layer)."""
     index = _matrix(w, "w", _DTYPES)
     n, k = w.shape
-    if n == 0:
-        raise ValueError("w: no rows")
+    if not 0 < n < _MAX:
+        raise ValueError(f"w: {n} rows")
     r, c = (k, n) if transpose else (n, k)
     out = Weight8(torch.empty(r, c, dtype=_E4M3, device=w.device),
                   torch.empty(_blocks(r), _blocks(c), dtype=_E8M0, device=w.device))
@@ -458,6 +459,8 @@ def _check_product(a: Act8, w: Weight8, bias, what: str, step: int):
     n, wk = w.codes.shape
     if wk != k:
         raise ValueError(f"w: shape {(n, wk)}, need [n, {k}]")
+    if m > _MAX or n > _MAX:
+        raise ValueError(f"{what}: {m} x {n} x {k} is too large")
     if n == 0 or n % step or k % 16:
         raise ValueError(f"{what} needs n % {step} == 0 and k % 16 == 0, got n {n}, k {k}")
     _matrix(w.scales, "w", (_E8M0,), (_blocks(n), _blocks(k)), index)
