@@ -177,20 +177,19 @@ TJ_DEV uint32_t pack_bf162(float a, float b) {
 TJ_DEV uint8_t* staged(uint8_t* buf, int lane, int j) { return buf + lane * 128 + ((j ^ (lane & 7)) << 4); }
 
 // gelu(x) = max(x, 0) - |x| T(|x|) exp(-x^2 / 2) for two values, where
-// T(a) = erfc(a / sqrt 2) exp(a^2 / 2) / 2 is a polynomial in t = 1 / (1 + 0.225 a):
-// fitted here (iterated weighted least squares over 0 <= a <= 9) to 3e-9 in
-// T exp(-a^2 / 2) and 1.1e-7 relative.  (The five terms of gelu_erf_x2, 7.5e-8
-// off, moved more codes over a boundary than the 32-bit sums do.)  Nothing
+// T(a) = erfc(a / sqrt 2) exp(a^2 / 2) / 2 is the polynomial of tj_act8.cuh.
+// (The five terms of gelu_erf_x2, 7.5e-8 off, moved more codes over a boundary
+// than the 32-bit sums do; with them the kernel took 47 us for 52.)  Nothing
 // cancels for x < 0.  Both reciprocals come from that of the product,
 // 1 / d0 = d1 / (d0 d1): the SFU takes 8 cycles an operation and warp.
 TJ_DEV uint64_t gelu8_x2(uint64_t x) {
   const float2 v = f32x2_split(x);
-  const float d0 = fmaf(fabsf(v.x), 0.225f, 1.f), d1 = fmaf(fabsf(v.y), 0.225f, 1.f);
+  // fminf turns a NaN into a number here, so that it stays out of its neighbour's reciprocal
+  const float d0 = fmaf(fminf(fabsf(v.x), 1e18f), kTailStep, 1.f), d1 = fmaf(fminf(fabsf(v.y), 1e18f), kTailStep, 1.f);
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d0 * d1));
   const uint64_t t = f32x2(r * d1, r * d0);
-  constexpr float kC[8] = {0.09031444994160742f, 0.08178340952580349f, 0.1346013969305005f, -0.09456394526861704f,
-                           0.4214357682285032f, -0.4126644252272553f, 0.37029267947368516f, -0.09119933652481564f};
+  constexpr float kC[8] = TJ_TAIL_COEFS;
   uint64_t q = f32x2(kC[7], kC[7]);
 #pragma unroll
   for (int i = 6; i >= 0; --i) q = ffma_x2(t, q, f32x2(kC[i], kC[i]));

@@ -434,6 +434,28 @@ def test_ffn_in(m, n, k, scale):
         close(back, want, 1.07 * err + 2.0 ** -4 * torch.maximum(want.abs(), 2.0 ** -6 * scale_of))
 
 
+@pytest.mark.parametrize("m,n", [(40, 256), (2304, 2304)])
+def test_nan_stays_in_its_column(m, n):
+    """A NaN in one weight row is that column's alone, in the product and in both GELU outputs (CTA and pair kernels)."""
+    a, w = rnd((m, 256), 1), rnd((n, 256), 2, scale=0.1)
+    w[33, 7] = math.nan
+    w[34, 200] = math.inf
+    a8, w8 = ops.checkpoint8(a.to(DEV)), ops.pack_weight8(w.to(DEV))
+    clean = w.clone()
+    clean[33:35] = 0
+    c8 = ops.pack_weight8(clean.to(DEV))
+    bad = torch.zeros(n, dtype=torch.bool)
+    bad[33:35] = True
+    for out in F:
+        got = ops.gemm8(a8, w8, out_dtype=out).cpu()
+        assert torch.isnan(got[:, bad]).all() and not torch.isnan(got[:, ~bad]).any()
+    for got, want in zip(ops.gemm8_gelu(a8, w8), ops.gemm8_gelu(a8, c8)):
+        got, want = ops.restore8(got, torch.float32).cpu(), ops.restore8(want, torch.float32).cpu()
+        assert torch.isnan(got[:, bad]).all() and not torch.isnan(got[:, ~bad]).any()
+        assert torch.equal(got[:, 128:], want[:, 128:])
+    assert ops.device_error() == 0
+
+
 # ---------------------------------------------------------------- weight gradient
 @pytest.mark.parametrize("rows,n,k", [(1, 8, 16), (64, 256, 256), (65, 264, 272), (633, 1000, 528), (1500, 256, 512),
                                       (5000, 512, 256), (130, 2048, 1024)])
