@@ -4,7 +4,8 @@ Public surface:
     techjam_b200.dispatcher.CANDIDATE          candidate spec (reference ``--candidate`` API)
     techjam_b200.dispatcher.DispatchingTransformer
     techjam_b200.model.B200Transformer          nn.Module with the reference parameter tree
-    techjam_b200.ops                            kernel-level building blocks (torch tensors in/out)
+    techjam_b200.ops                            kernel-level building blocks (torch tensors in/out), and the
+                                                training and 8-bit operators (layernorm_train, gemm8, ...)
     techjam_b200.build.build()                  compile libtj.so in-tree
 """
 

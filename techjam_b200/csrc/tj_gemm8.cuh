@@ -665,8 +665,9 @@ struct Gemm8PairCfg {
   static constexpr int kSfSlots = 2;
   static constexpr int kSfCols = 12;  // 4 for A's 128 rows, 8 for W's 256
   static constexpr int kThreads = 256 + 32 * kEpiWarps;
-  static constexpr int kRegLaunch = KIND == kG8Gelu ? 80 : 128;  // kG8Gelu: warpgroups with 24 + 40 + 4 * 104 (96: 55 us for 47)
-  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kStagingBytes + 256;
+  // kG8Gelu: warpgroups with 24 + 40 + 4 * 104 (96: 55 us for 47); kG8F32: 56 + 56 + 2 * 200
+  static constexpr int kRegLaunch = KIND == kG8Gelu ? 80 : 128;
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kStagingBytes + 512;
   static_assert(kSmemBytes <= 232448, "shared memory");
 };
 
@@ -687,7 +688,6 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
     gemm8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                       const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ CUtensorMap tmAux,
                       const Gemm8Params p) {
-  static_assert(KIND == kG8F16 || KIND == kG8BF16 || KIND == kG8Gelu, "kind");
   using Cfg = Gemm8PairCfg<KIND>;
   constexpr int S = Cfg::kStages, SF = Cfg::kSfSlots;
   extern __shared__ uint8_t smem_raw[];
@@ -702,6 +702,7 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
   uint64_t* sf_empty = sf_full + SF;      // [SF]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sf_empty + SF);
   volatile uint8_t* agreed = reinterpret_cast<volatile uint8_t*>(tmem_slot + 1);  // kG8Gelu: [2][16], an epilogue warp's wait succeeded
+  uint64_t* res_full = full + 32;  // kG8F32: [8 epilogue warps][2]
   static_assert((2 * S + 5 + 2 * SF) * 8 + 4 + 32 <= 256, "barrier space");
 
   const int warp = threadIdx.x >> 5;
@@ -713,6 +714,8 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
     for (int i = 0; i < 2; ++i) { mbar_init(acc_full + i, 1); mbar_init(acc_empty + i, 2 * Cfg::kEpiWarps); }
     mbar_init(shared_free, 8);
     for (int i = 0; i < SF; ++i) { mbar_init(sf_full + i, 8); mbar_init(sf_empty + i, 1); }
+    if constexpr (KIND == kG8F32)
+      for (int i = 0; i < 16; ++i) mbar_init(res_full + i, 1);
     fence_mbar_init();
   }
   if (warp == 2) {
@@ -728,7 +731,7 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
   const int m_tiles = (p.M + 255) / 256;
   const long long total = (long long)m_tiles * n_tiles;
   const int kblocks = p.kblocks;
-  constexpr int kChunk = KIND == kG8Gelu ? kG8Chunk : 1 << 30;
+  constexpr int kChunk = KIND == kG8F32 || KIND == kG8Gelu ? kG8Chunk : 1 << 30;
   // both CTAs take or leave a tile together
   auto pair_has_rows = [&](int mt) {
     return tile_has_rows(p.mask, mt * 256, p.M, lane) || tile_has_rows(p.mask, mt * 256 + 128, p.M, lane);
@@ -736,6 +739,7 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
 
   if (warp < 4) {
     if constexpr (KIND == kG8Gelu) reg_dealloc<24>();
+    if constexpr (KIND == kG8F32) reg_dealloc<56>();
     if (warp == 0) {
       // ---------------------------------------------------------- TMA producer
       if (lane == 0) { tma_prefetch_desc(&tmA); tma_prefetch_desc(&tmW); }
@@ -810,6 +814,7 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
   } else if (warp < 8) {
     // ------------------------------------------------------------ scales -> TMEM
     if constexpr (KIND == kG8Gelu) reg_dealloc<40>();
+    if constexpr (KIND == kG8F32) reg_dealloc<56>();
     // The words of a group of four K blocks are on their way a group ahead,
     // across tiles, so that no slot waits for global memory.
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -860,6 +865,7 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
   } else {
     // ------------------------------------------------------------ epilogue
     if constexpr (KIND == kG8Gelu) reg_alloc<104>();
+    if constexpr (KIND == kG8F32) reg_alloc<200>();
     const int ew = warp - 8, quarter = warp & 3;
     constexpr int kGroups = Cfg::kEpiWarps / 4, kCW = 256 / kGroups;
     const int cg = ew >> 2;  // column group
@@ -868,6 +874,7 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
     const uint32_t acc_empty0 = map_to_rank(acc_empty, 0), shared_free0 = map_to_rank(shared_free, 0);
     uint32_t used = 0;  // staging buffers used so far
     int turn = 0;       // kG8Gelu: set of flags of this tile
+    uint32_t rphase = 0;  // kG8F32: bit b: parity of buffer b's next residual load
     int abuf = 0;
     uint32_t aphase = 0;
     bool ok = true;
@@ -956,6 +963,102 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
             }
           }
         }
+      } else if constexpr (KIND == kG8F32) {
+        // 128 columns as four 32-column (128-byte) pieces; the residual comes
+        // into the staging buffers two pieces ahead of its use
+        const int pieces = row0 < p.M ? max(0, min(4, (p.N - col0 + 31) / 32)) : 0;
+        const bool fetch = p.has_resid && live;
+        auto load_resid = [&](int c) {  // lane 0; its buffer's store has been read
+          const uint32_t b = (used + c) & 1;
+          mbar_expect_tx(res_full + 2 * ew + b, 4096);
+          tma_load_2d(bufs + b * 4096, &tmAux, res_full + 2 * ew + b, col0 + 32 * c, row0);
+        };
+        if (fetch && lane == 0) {
+          bulk_wait_read<0>();
+          for (int c = 0; c < min(2, pieces); ++c) load_resid(c);
+        }
+        __syncwarp();
+        float acc[128];
+#pragma unroll
+        for (int i = 0; i < 128; ++i) acc[i] = 0.f;
+        if (live) {
+          for (int kb = 0; kb < kblocks; kb += kChunk) {
+            if (!wait_acc()) break;  // on to the residual's own waits, so that no load is in flight at the end
+            const uint32_t taddr = acc_addr();
+            uint32_t r[32];
+            // buffer 0 shares its last 32 columns (group 1's last piece), buffer 1 its first
+            const bool swap = abuf == 0 && cg == 1;
+            const bool mine = swap || (abuf == 1 && cg == 0);
+            auto add = [&](float* a) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) a[i] += __uint_as_float(r[i]);
+            };
+            if (swap) {
+              tmem_ld32(taddr + 96, r);
+              tmem_ld_wait();
+              free_shared();
+              add(acc + 96);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              if (c == 3 && swap) continue;  // warp-uniform
+              tmem_ld32(taddr + 32 * c, r);
+              tmem_ld_wait();
+              if (c == 0 && mine && !swap) free_shared();
+              add(acc + 32 * c);
+            }
+            free_acc();
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (c < pieces) {
+            const int col = col0 + 32 * c;
+            const uint32_t b = (used + c) & 1;
+            uint8_t* buf = bufs + b * 4096;
+            if (fetch) {
+              uint64_t* bar = res_full + 2 * ew + b;
+              if (!mbar_wait_warp(bar, (rphase >> b) & 1u, p.err, kErrGemm8Epilogue)) {
+                ok = false;
+                mbar_drain(bar, 1, 1, (rphase >> b) & 1u);
+              }
+              rphase ^= 1u << b;
+            } else {
+              if (lane == 0) bulk_wait_read<1>();
+              __syncwarp();
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              float4* dst = reinterpret_cast<float4*>(staged(buf, lane, j));
+              float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (valid) {
+                o = make_float4(acc[32 * c + 4 * j], acc[32 * c + 4 * j + 1], acc[32 * c + 4 * j + 2],
+                                acc[32 * c + 4 * j + 3]);
+                if (p.bias != nullptr && col + 4 * j < p.N) {
+                  const float4 bb = __ldg(reinterpret_cast<const float4*>(p.bias + col) + j);
+                  o.x += bb.x; o.y += bb.y; o.z += bb.z; o.w += bb.w;
+                }
+                if (p.has_resid) {
+                  const float4 rr = *dst;
+                  o.x += rr.x; o.y += rr.y; o.z += rr.z; o.w += rr.w;
+                }
+              }
+              *dst = o;
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tmOut, buf, col, row0);
+              bulk_commit();
+              if (fetch && c + 2 < pieces) {
+                bulk_wait_read<0>();
+                load_resid(c + 2);
+              }
+            }
+            __syncwarp();
+          }
+        }
+        used += pieces;
       } else {
         if (live && !wait_acc()) break;
         const int cur = abuf;

@@ -168,14 +168,15 @@ int launch_gemm8_pair(const Gemm8Args& g, const tj::Gemm8Params& p, int dev, cud
   static int max_pairs[64] = {};
   PairLaunch l(Cfg::kThreads, Cfg::kSmemBytes, st);
   int pairs = 0;
-  TJH_CHECK(cluster_pairs(kern, l.cfg, KIND == tj::kG8Gelu ? Cfg::kRegLaunch : 0, dev, max_pairs, mu, &pairs));
+  TJH_CHECK(cluster_pairs(kern, l.cfg, KIND == tj::kG8Gelu || KIND == tj::kG8F32 ? Cfg::kRegLaunch : 0, dev, max_pairs, mu, &pairs));
   CUtensorMap ta, tw, to, tx;
   TJH_CHECK(tj_host::make_map(&ta, g.a, 1, p.M, p.K, 128, 128));
   TJH_CHECK(tj_host::make_map(&tw, g.w, 1, p.N, p.K, 128, 128));
-  constexpr int elt = KIND == tj::kG8Gelu ? 1 : 2;
+  constexpr int elt = KIND == tj::kG8Gelu ? 1 : (KIND == tj::kG8F32 ? 4 : 2);
   TJH_CHECK(tj_host::make_map(&to, g.out, elt, p.M, p.N, 32, 128 / elt));
   tx = to;
   if (KIND == tj::kG8Gelu) TJH_CHECK(tj_host::make_map(&tx, g.aux_out, 1, p.M, p.N, 32, 128));
+  else if (g.aux_in != nullptr) TJH_CHECK(tj_host::make_map(&tx, g.aux_in, 4, p.M, p.N, 32, 32));
   const long long tiles = (long long)((p.M + 255) / 256) * ((p.N + 255) / 256);
   l.cfg.gridDim = dim3(2 * (unsigned)std::min<long long>(tiles, pairs));
   TJH_CUDA(cudaLaunchKernelEx(&l.cfg, kern, ta, tw, to, tx, p));
@@ -199,11 +200,12 @@ int gemm8_params(tj::Gemm8Params* p, const void* a, const uint8_t* as, const voi
 
 template <int KIND>
 int gemm8_kind(const Gemm8Args& g, const tj::Gemm8Params& p, int dev, int sms, cudaStream_t st) {
-  if constexpr (KIND != tj::kG8F32) {
-    // 256 x 256 tiles of CTA pairs once they fill the GPU
-    const long long pair_tiles = (long long)((p.M + 255) / 256) * ((p.N + 255) / 256);
-    if (2 * pair_tiles >= sms) return launch_gemm8_pair<KIND>(g, p, dev, st);
-  }
+  // 256 x 256 tiles of CTA pairs once they fill the GPU.  A 32-bit result with
+  // a short sum is bound by its bytes, and the single CTAs' deeper staging
+  // moves them better (32768 x 4096 x 1024, residual: 261 us for 266; but
+  // 32768 x 1024 x 4096: 184 for 158, and 16384 x 2048 x 2048: 108 for 103).
+  const long long pair_tiles = (long long)((p.M + 255) / 256) * ((p.N + 255) / 256);
+  if (2 * pair_tiles >= sms && (KIND != tj::kG8F32 || p.kblocks >= 16)) return launch_gemm8_pair<KIND>(g, p, dev, st);
   if constexpr (KIND != tj::kG8Gelu) {
     // few tiles: half as wide, so that twice as many SMs share the weight's bytes
     const long long tiles = (long long)((p.M + 127) / 128) * ((p.N + 127) / 128);
