@@ -18,6 +18,8 @@ Contents
                      score-spread guard, restated from
                      ``src/implementations/poly_reference.py`` and
                      ``src/implementations/poly_guard.py``.
+``act8``             8-bit activations and the training operators in 64 bits
+                     (no counterpart in the reference).
 
 Parity of this restatement is pinned by the golden fixtures in
 ``tests/golden/`` (generated by ``tests/golden/make_golden.py`` from the
