@@ -178,23 +178,22 @@ TJ_DEV uint8_t* staged(uint8_t* buf, int lane, int j) { return buf + lane * 128 
 
 // gelu(x) = max(x, 0) - |x| T(|x|) exp(-x^2 / 2) for two values, where
 // T(a) = erfc(a / sqrt 2) exp(a^2 / 2) / 2 is the polynomial of tj_act8.cuh.
-// (The five terms of gelu_erf_x2, 7.5e-8 off, moved more codes over a boundary
-// than the 32-bit sums do; with them the kernel took 47 us for 52.)  Nothing
-// cancels for x < 0.  Both reciprocals come from that of the product,
-// 1 / d0 = d1 / (d0 d1): the SFU takes 8 cycles an operation and warp.
+// Nothing cancels for x < 0.  exp(-x^2 / 2) = 2^-((x log2(e) / 2) x): rounded
+// twice where the square of x sqrt(log2(e) / 2) counts its rounding twice.  A
+// reciprocal for each value keeps a value's result its own; one of the product
+// for both took as long (16384 x 2048 x 512: 55 us a call) and cost bits.  For
+// |x| near the largest float t flushes to zero and the exponential is zero.
 TJ_DEV uint64_t gelu8_x2(uint64_t x) {
   const float2 v = f32x2_split(x);
-  // fminf turns a NaN into a number here, so that it stays out of its neighbour's reciprocal
-  const float d0 = fmaf(fminf(fabsf(v.x), 1e18f), kTailStep, 1.f), d1 = fmaf(fminf(fabsf(v.y), 1e18f), kTailStep, 1.f);
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d0 * d1));
-  const uint64_t t = f32x2(r * d1, r * d0);
-  constexpr float kC[8] = TJ_TAIL_COEFS;
-  uint64_t q = f32x2(kC[7], kC[7]);
+  float t0, t1;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(fmaf(fabsf(v.x), kTailStep, 1.f)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(fmaf(fabsf(v.y), kTailStep, 1.f)));
+  const uint64_t t = f32x2(t0, t1);
+  constexpr float kC[kTailTerms] = TJ_TAIL_COEFS;
+  uint64_t q = f32x2(kC[kTailTerms - 1], kC[kTailTerms - 1]);
 #pragma unroll
-  for (int i = 6; i >= 0; --i) q = ffma_x2(t, q, f32x2(kC[i], kC[i]));
-  const uint64_t y = fmul_x2(x, f32x2(0.84932180028801904f, 0.84932180028801904f));  // sqrt(log2(e) / 2)
-  const float2 yy = f32x2_split(fmul_x2(y, y));
+  for (int i = kTailTerms - 2; i >= 0; --i) q = ffma_x2(t, q, f32x2(kC[i], kC[i]));
+  const float2 yy = f32x2_split(fmul_x2(fmul_x2(x, f32x2(0.72134752044448170f, 0.72134752044448170f)), x));  // log2(e) / 2
   const float2 tail = f32x2_split(fmul_x2(fmul_x2(t, q), f32x2(fast_exp2(-yy.x), fast_exp2(-yy.y))));
   return f32x2(fmaf(-fabsf(v.x), tail.x, fmaxf(v.x, 0.f)), fmaf(-fabsf(v.y), tail.y, fmaxf(v.y, 0.f)));
 }
@@ -209,8 +208,9 @@ TJ_DEV uint32_t e4m3_pairs(uint64_t x, uint64_t y, uint64_t inv) {
 // piece `piece0` on, and the block's scale bytes (rows that are not valid:
 // zeros).  join(a, b) takes the maxima with the other half's.
 // gelu grows with h > 0 and its dip for h < 0 is 0.17 deep, which gelu(0.3)
-// exceeds: above that the largest |g| is gelu of the largest h, and only a
-// warp with a smaller one looks at every g.  Called by whole warps.
+// exceeds: above that the largest |g| is gelu of the largest h (as computed
+// too: no smaller h comes out on the other side of any scale's border), and
+// only a warp with a smaller one looks at every g.  Called by whole warps.
 template <int N, typename Join>
 TJ_DEV void gelu_pack_row(uint64_t (&h)[N / 2], bool valid, uint8_t* bufg, uint8_t* bufh, int piece0, int lane,
                           uint32_t& gbyte, uint32_t& hbyte, Join&& join) {
