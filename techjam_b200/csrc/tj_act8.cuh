@@ -361,40 +361,49 @@ constexpr int kTailTerms = 9;
    0.051166784f}
 
 // d gelu(h) / dh = Phi(h) + h phi(h), Phi the normal distribution and phi its
-// density, for the exact (erf) GELU; two values at a time.  Odd about 1/2:
-// with a = |h| and u = exp(-a^2 / 2),
-//   slope = 1/2 + sign(h) (1/2 - erfc(a / sqrt 2) / 2 + a u / sqrt(2 pi)),
-// and one exponential serves both terms.  z = a sqrt(log2(e) / 2) makes
-// u = 2^(-z^2).  min.NaN keeps a NaN and makes an infinity finite, so that a u
-// is 0 and not NaN.
+// density, for the exact (erf) GELU; two values at a time.  With a = |h|,
+// u = exp(-a^2 / 2) and v = u (a / sqrt(2 pi) - erfc(a / sqrt 2) exp(a^2 / 2) / 2)
+// it is 1 + v for h >= 0 and -v for h < 0 (formed as 1/2 - (1/2 + v) it loses
+// the tail, all of it at h = -7), and one exponential serves both terms of v.
+// What 32 bits keep: 2e-7 for h > -1, and below it 6e-7 of the value to -3,
+// 1.4e-6 to -5, 3.4e-6 to -9 (a plain evaluation: 6e-7, 7e-7, 2.1e-6), from
+// the roundings of a^2 / 2.  min.NaN keeps a NaN and makes an infinity finite,
+// so that a u is 0 and not NaN.
 TJ_DEV float2 gelu_slope_x2(float h0, float h1) {
   float a0, a1;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(a0) : "f"(fabsf(h0)), "f"(1e18f));
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(a1) : "f"(fabsf(h1)), "f"(1e18f));
-  constexpr float kZ = 0.84932180028801904f;  // sqrt(log2(e) / 2)
   constexpr float kC[kTailTerms] = TJ_TAIL_COEFS;
-  const uint64_t z = fmul_x2(f32x2(a0, a1), f32x2(kZ, kZ));
-  const float2 den = f32x2_split(ffma_x2(z, f32x2(kTailStep / kZ, kTailStep / kZ), f32x2(1.f, 1.f)));
-  const float2 zz = f32x2_split(fmul_x2(z, z));
+  const uint64_t a = f32x2(a0, a1);
+  const float2 den = f32x2_split(ffma_x2(a, f32x2(kTailStep, kTailStep), f32x2(1.f, 1.f)));
+  const float2 aa = f32x2_split(fmul_x2(fmul_x2(a, f32x2(0.72134752044448170f, 0.72134752044448170f)), a));  // log2(e) / 2
   // a reciprocal each: one of the product for both costs three products and
   // keeping a NaN from its neighbour (143 us for 137 at 32768 x 4096 bf16)
   float t0, t1;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t0) : "f"(den.x));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t1) : "f"(den.y));
-  const uint64_t t = f32x2(t0, t1), u = f32x2(fast_exp2(-zz.x), fast_exp2(-zz.y));
-  uint64_t q = f32x2(-kC[kTailTerms - 1], -kC[kTailTerms - 1]);  // the negative polynomial, so that the sums are plain fused multiply-adds
+  const uint64_t t = f32x2(t0, t1), u = f32x2(fast_exp2(-aa.x), fast_exp2(-aa.y));
+  uint64_t q = f32x2(kC[kTailTerms - 1], kC[kTailTerms - 1]);
 #pragma unroll
-  for (int i = kTailTerms - 2; i >= 0; --i) q = ffma_x2(t, q, f32x2(-kC[i], -kC[i]));
-  const uint64_t inner = ffma_x2(z, f32x2(0.39894228040143268f / kZ, 0.39894228040143268f / kZ), fmul_x2(t, q));
-  const float2 m = f32x2_split(ffma_x2(u, inner, f32x2(0.5f, 0.5f)));
-  return make_float2(0.5f + copysignf(m.x, h0), 0.5f + copysignf(m.y, h1));
+  for (int i = kTailTerms - 2; i >= 0; --i) q = ffma_x2(t, q, f32x2(kC[i], kC[i]));
+  // -v; the 1 is then added under a predicate (a select after both sums: 141 us for 137)
+  float2 m = f32x2_split(fmul_x2(u, ffma_x2(a, f32x2(-0.39894228040143268f, -0.39894228040143268f), fmul_x2(t, q))));
+  asm("{.reg .pred p; setp.ge.f32 p, %1, 0f00000000; @p sub.f32 %0, 0f3F800000, %0;}" : "+f"(m.x) : "f"(h0));
+  asm("{.reg .pred p; setp.ge.f32 p, %1, 0f00000000; @p sub.f32 %0, 0f3F800000, %0;}" : "+f"(m.y) : "f"(h1));
+  return m;
 }
+
+// CTAs per SM of the packing forms of 16-bit gradients, left to the compiler
+// otherwise (16384 x 4096, 8-bit h: 96 us bf16 and 94 fp16 for 102 and 102; h
+// in 16 bits: 94 and 102 for 113 and 109, 6 CTAs 109 and 143).
+template <typename T, bool H8, bool PACK>
+constexpr int gelu_bwd_ctas() { return sizeof(T) == 2 && PACK ? (H8 ? 6 : 5) : 0; }
 
 // dh = dy * gelu'(h), rounded to T; PACK: also the 8-bit form of the rounded
 // dh, so that the packed copy is the one that packing dh would give.
 // h: 8-bit copy (H8) or a tensor of type T.
 template <typename T, bool H8, bool PACK, bool VEC>
-__global__ void __launch_bounds__(256) gelu_bwd_kernel(const T* __restrict__ dy, const void* __restrict__ h,
+__global__ void __launch_bounds__(256, gelu_bwd_ctas<T, H8, PACK>()) gelu_bwd_kernel(const T* __restrict__ dy, const void* __restrict__ h,
                                                        const uint8_t* __restrict__ h_scales, long long rows, int cols,
                                                        const uint8_t* __restrict__ mask, T* __restrict__ dh,
                                                        uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {

@@ -63,3 +63,37 @@ def test_gelu_product_changes_no_more_codes_than_plain_32_bits():
     assert ops.device_error() == 0
     for key, (own, plain) in changed.items():
         assert own <= 1.2 * plain, (key, own, plain)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16, torch.bfloat16])
+def test_gelu_slope_keeps_its_tail(dt):
+    """h in [-9, -1], relative to the slope itself: for a = |h| the exponent
+    a^2 / 2 is rounded three times (constant, product, product: at most
+    3 a^2 / 2 u), the exponential is 4 u off, and the rest (t with 4 u, nine
+    terms whose magnitudes add up to 4 times their sum at most, two products
+    and a difference of which the smaller term is at most 0.86) counts below
+    60 u for a <= 1.5 and falls; then the product with dy and the output."""
+    u = 2.0 ** -24
+    h = -torch.linspace(1.0, 9.0, 100 * 1001, device=DEV).view(100, 1001)
+    h = h.to(dt)
+    dy = rnd(h.shape, 3).to(dt)
+    x = h.double()
+    slope = 0.5 * torch.special.erfc(-x / math.sqrt(2.0)) + x * torch.exp(-x * x / 2) / math.sqrt(2 * math.pi)
+    want = dy.double() * slope
+    f = torch.finfo(dt)
+    tol = ((1.5 * x * x + 66) * u + f.eps / 2) * want.abs() + f.smallest_normal * f.eps / 2
+    got = ops.gelu_backward(dy, h).double()
+    assert torch.all((got - want).abs() <= tol), float(((got - want).abs() / tol).max())
+
+
+def test_gelu_slope_packed_tail():
+    """A block of far negative values gets the scale and the codes of its own values."""
+    h = -torch.linspace(6.0, 9.0, 64 * 128, device=DEV).view(64, 128)
+    dy = torch.ones_like(h)
+    dh, dh8 = ops.gelu_backward(dy, h, pack=True)
+    x = h.double()
+    want = 0.5 * torch.special.erfc(-x / math.sqrt(2.0)) + x * torch.exp(-x * x / 2) / math.sqrt(2 * math.pi)
+    assert torch.equal(values(dh8), in_8_bits(dh.double()))
+    # half a step of a code with 3 fraction bits, or of the smallest under the row's scale (2^-10 of 2^-8 of its maximum)
+    tol = (2.0 ** -4 + 1e-4) * want.abs() + 2.0 ** -17 * want.abs().amax(1, keepdim=True)
+    assert torch.all((values(dh8) - want).abs() <= tol)
