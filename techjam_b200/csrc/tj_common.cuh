@@ -17,6 +17,7 @@
 #ifndef TJ_WAIT_NS
 #define TJ_WAIT_NS 4000000000ull  // 4 s: far above any legitimate stall
 #endif
+#define TJ_DRAIN_NS 10000000ull  // 10 ms
 
 namespace tj {
 
@@ -91,14 +92,23 @@ TJ_DEV bool error_raised(const int* err) { return *reinterpret_cast<const volati
 TJ_DEV bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* err, int site) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, site));
 }
-// After an expired wait: the loads of a ring of n stages, issued up to (not
-// including) `stage` of pass `phase`, have landed (or the limit is reached)
-// before the thread goes on to leave the kernel.
-TJ_DEV void mbar_drain(uint64_t* full, int n, int stage, uint32_t phase) {
-  for (int i = 0; i < n; ++i)
-    for (int k = 0; k < (1 << 16) && !mbar_try_wait(full + i, i < stage ? phase : phase ^ 1u); ++k) {
+// What a thread set going asynchronously is over before it goes on to leave
+// the kernel: it waits for its barriers' last phases, and where an expired wait
+// has kept one from completing, until TJ_DRAIN_NS have passed since (a load or
+// an MMA takes microseconds).  No error: whoever gave up has recorded it.
+struct Drain {
+  uint64_t t0 = 0;
+  TJ_DEV void wait(uint64_t* bar, uint32_t parity) {
+    while (!mbar_try_wait(bar, parity)) {
+      if (t0 == 0) t0 = global_ns();
+      if (global_ns() - t0 > TJ_DRAIN_NS) return;
     }
-}
+  }
+  // A ring of n stages used up to (not including) `stage` of pass `phase`.
+  TJ_DEV void ring(uint64_t* bars, int n, int stage, uint32_t phase) {
+    for (int i = 0; i < n; ++i) wait(bars + i, i < stage ? phase : phase ^ 1u);
+  }
+};
 // Plain arrive by one lane of a converged warp (barriers counting warps).
 TJ_DEV void mbar_arrive_elect(uint64_t* bar) {
   asm volatile(
@@ -260,6 +270,15 @@ TJ_DEV void umma_commit_pair_both_elect(uint64_t* bar) {
       "elect.sync r|e, 0xffffffff;\n\t"
       "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
       ::"r"(smem_u32(bar)), "h"((uint16_t)0x3)
+      : "memory");
+}
+
+// The even CTA's copy alone.
+TJ_DEV void umma_commit_pair_elect(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t.reg .b32 r;\n\t"
+      "elect.sync r|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
       : "memory");
 }
 

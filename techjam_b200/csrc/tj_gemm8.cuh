@@ -314,8 +314,9 @@ __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
   uint64_t* sf_full = acc_empty + 2;    // [SF]
   uint64_t* sf_empty = sf_full + SF;    // [SF]
   uint64_t* res_full = sf_empty + SF;   // [epilogue warps][bufs], kG8F32
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(res_full + (KIND == kG8F32 ? Cfg::kEpiWarps * Cfg::kBufs : 0));
-  static_assert((2 * S + 4 + 2 * SF + 32) * 8 + 4 <= 512, "barrier space");
+  uint64_t* drained = res_full + (KIND == kG8F32 ? Cfg::kEpiWarps * Cfg::kBufs : 0);  // every MMA is complete
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+  static_assert((2 * S + 5 + 2 * SF + 32) * 8 + 4 <= 512, "barrier space");
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -325,6 +326,7 @@ __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
     for (int i = 0; i < SF; ++i) { mbar_init(sf_full + i, 4); mbar_init(sf_empty + i, 1); }
     if constexpr (KIND == kG8F32)
       for (int i = 0; i < Cfg::kEpiWarps * Cfg::kBufs; ++i) mbar_init(res_full + i, 1);
+    mbar_init(drained, 1);
     fence_mbar_init();
   }
   if (warp == 2) {
@@ -363,7 +365,7 @@ __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
         if (++stage == S) { stage = 0; phase ^= 1u; }
       }
     }
-    if (!ok && lane == 0) mbar_drain(full, S, stage, phase);
+    if (lane == 0) Drain().ring(full, S, stage, phase);
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     int stage = 0, abuf = 0, slot = 0;
@@ -402,6 +404,9 @@ __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
         }
       }
     }
+    umma_commit_elect(drained);
+    Drain().wait(drained, 0);
+    __syncwarp();
   } else if (warp >= 4 && warp < 8) {
     // ------------------------------------------------------------ scales -> TMEM
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -509,7 +514,8 @@ __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
               uint64_t* bar = res_full + ew * Cfg::kBufs + b;
               if (!mbar_wait_warp(bar, (rphase >> b) & 1u, p.err, kErrGemm8Epilogue)) {
                 ok = false;
-                mbar_drain(bar, 1, 1, (rphase >> b) & 1u);
+                Drain().wait(bar, (rphase >> b) & 1u);
+                __syncwarp();
               }
               rphase ^= 1u << b;
             } else {
@@ -703,6 +709,7 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sf_empty + SF);
   volatile uint8_t* agreed = reinterpret_cast<volatile uint8_t*>(tmem_slot + 1);  // kG8Gelu: [2][16], an epilogue warp's wait succeeded
   uint64_t* res_full = full + 32;  // kG8F32: [8 epilogue warps][2]
+  uint64_t* drained = full + 48;   // every MMA is complete (even CTA's copy)
   static_assert((2 * S + 5 + 2 * SF) * 8 + 4 + 32 <= 256, "barrier space");
 
   const int warp = threadIdx.x >> 5;
@@ -716,6 +723,7 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
     for (int i = 0; i < SF; ++i) { mbar_init(sf_full + i, 8); mbar_init(sf_empty + i, 1); }
     if constexpr (KIND == kG8F32)
       for (int i = 0; i < 16; ++i) mbar_init(res_full + i, 1);
+    mbar_init(drained, 1);
     fence_mbar_init();
   }
   if (warp == 2) {
@@ -762,12 +770,8 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
         }
         ok = __all_sync(0xffffffffu, ok);
       }
-      // after an expired wait: give the last loads time to land
-      if (!ok && lane == 0) {
-        const uint64_t t = global_ns();
-        while (global_ns() - t < 100000) {
-        }
-      }
+      // the loads signal the even CTA, but both learn when the MMAs have used them
+      if (lane == 0) Drain().ring(empty, S, stage, phase);
     } else if (warp == 1 && rank == 0) {
       // ---------------------------------------------------------- MMA issuer
       int stage = 0, abuf = 0, slot = 0;
@@ -810,6 +814,9 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
           }
         }
       }
+      umma_commit_pair_elect(drained);
+      Drain().wait(drained, 0);
+      __syncwarp();
     }
   } else if (warp < 8) {
     // ------------------------------------------------------------ scales -> TMEM
@@ -1020,7 +1027,8 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
               uint64_t* bar = res_full + 2 * ew + b;
               if (!mbar_wait_warp(bar, (rphase >> b) & 1u, p.err, kErrGemm8Epilogue)) {
                 ok = false;
-                mbar_drain(bar, 1, 1, (rphase >> b) & 1u);
+                Drain().wait(bar, (rphase >> b) & 1u);
+                __syncwarp();
               }
               rphase ^= 1u << b;
             } else {

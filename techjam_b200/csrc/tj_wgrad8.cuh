@@ -152,7 +152,8 @@ __global__ void __launch_bounds__(kWgThreads, 1)
   uint64_t* empty = cleared + S;    // [S]
   uint64_t* acc_full = empty + S;     // [2]
   uint64_t* acc_empty = acc_full + 2; // [2] (even CTA's copy is the live one)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* drained = acc_empty + 2;  // every MMA is complete (even CTA's copy)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -167,6 +168,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
       mbar_init(empty + i, 1);
     }
     for (int i = 0; i < 2; ++i) { mbar_init(acc_full + i, 1); mbar_init(acc_empty + i, 16); }
+    mbar_init(drained, 1);
     fence_mbar_init();
   }
   if (warp == 2) {
@@ -229,14 +231,8 @@ __global__ void __launch_bounds__(kWgThreads, 1)
           if (++stage == S) { stage = 0; phase ^= 1u; }
         }
       }
-      // after an expired wait: the last loads were issued before a wait that
-      // took the limit or saw another warp's, and every MMA that could read
-      // them is past; give them time to land
-      if (!ok) {
-        const uint64_t t = global_ns();
-        while (global_ns() - t < 100000) {
-        }
-      }
+      // the loads signal the even CTA, but both learn when the MMAs have used them
+      Drain().ring(empty, S, stage, phase);
     } else if (warp == 1 && rank == 0) {
       // ---------------------------------------------------------- MMA issuer
       constexpr uint32_t idesc =
@@ -274,6 +270,9 @@ __global__ void __launch_bounds__(kWgThreads, 1)
           }
         }
       }
+      umma_commit_pair_elect(drained);
+      Drain().wait(drained, 0);
+      __syncwarp();
     } else if (warp == 2 && p.list != nullptr) {
       // ---------------------------------------------------------- masked tokens of dY's tile
       const uint32_t cleared0 = map_to_rank(cleared, 0);

@@ -1,0 +1,51 @@
+"""Bounded waits of the 8-bit product on the GPU, without a fault: with a limit
+of next to nothing a wait gives up after 64 tries (0.27 ms), which a sum over
+262144 columns outlasts.  The kernel then records the site, leaves with nothing
+in flight, and the same call with the default limit is right."""
+
+import pytest
+import torch
+
+from techjam_b200 import _lib, ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+K = 262144
+SITES = range(401, 405)
+
+
+def ones(rows, exponent):
+    """Codes of 1.0 under the scale 2^exponent."""
+    codes = torch.full((rows, K), 0x38, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
+    return codes, exponent + 127
+
+
+def operands(m, n):
+    a, ae = ones(m, -9)
+    w, we = ones(n, -9)
+    scale = lambda rows, byte: torch.full((rows, K // 128), byte, dtype=torch.uint8, device=DEV).view(torch.float8_e8m0fnu)
+    return ops.Act8(a, scale(m, ae), torch.float16), ops.Weight8(w, scale((n + 127) // 128, we))
+
+
+# one tile of a single CTA; three tiles a CTA pair, so that loads, scales and MMAs wait for the epilogue that left
+@pytest.mark.parametrize("m,n", [(128, 64), (3840, 3840)])
+def test_expired_wait_leaves_in_order(m, n):
+    a, w = operands(m, n)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    ops.gemm8(a, w, out_dtype=torch.bfloat16, err=err)
+    assert int(err) == 0
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    _lib.call("tj_set_wait_limit", 1)
+    try:
+        start.record()
+        ops.gemm8(a, w, out_dtype=torch.bfloat16, err=err)
+        end.record()
+        torch.cuda.synchronize()
+    finally:
+        _lib.call("tj_set_wait_limit", 0)
+    assert int(err) in SITES
+    assert start.elapsed_time(end) < 1000
+    err.zero_()
+    # 262144 * 2^-18, exact in the accumulator
+    assert torch.all(ops.gemm8(a, w, out_dtype=torch.bfloat16, err=err) == 1)
+    assert int(err) == 0
