@@ -367,8 +367,9 @@ TJ_API int tj_gelu_backward(const void* dy, int dtype, const void* h, const uint
 
 /* out[m, n] = a[m, k] x w[n, k]^T [+ bias[n]] [+ resid[m, n]] on 8-bit
    operands, FP32 sums; resid (FP32) only with out_dtype TJ_F32, and it may
-   alias out.  k % 16 == 0, n % 8 == 0.  err: an int that is zero, set to a
-   site code (401-404) when a bounded wait expires. */
+   alias out.  k % 16 == 0, n % 8 == 0.  err: an int, set to a site code
+   (401-404) when it is zero and a bounded wait expires; what it holds before
+   changes nothing else, so calls may share one. */
 TJ_API int tj_gemm8(const void* a, const uint8_t* a_scales, const void* w, const uint8_t* w_scales, const float* bias,
                     int m, int n, int k, const uint8_t* mask, const float* resid, void* out, int out_dtype, int* err,
                     void* stream);

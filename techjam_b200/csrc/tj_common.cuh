@@ -5,7 +5,8 @@
 // TJ_WAIT_NS unless the host set another limit) the waiting thread records a
 // site code in the device error word and returns false; the kernel then
 // unwinds (releasing TMEM) instead of hanging the GPU.  Any CTA that finds the
-// error word already set bails out at its next wait.
+// error word already set bails out at its next wait; the kernels whose word
+// outlives a call (8-bit products, weight gradient) do not look at it.
 #pragma once
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -70,7 +71,9 @@ TJ_DEV bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// Bounded wait for the phase with the given parity to complete.
+// Bounded wait for the phase with the given parity to complete.  kSharedWord:
+// the word may hold an earlier call's error, which is none of this call's.
+template <bool kSharedWord = false>
 TJ_DEV bool mbar_wait(uint64_t* bar, uint32_t parity, int* err, int site) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = global_ns();
@@ -78,7 +81,7 @@ TJ_DEV bool mbar_wait(uint64_t* bar, uint32_t parity, int* err, int site) {
   for (uint32_t i = 1;; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((i & 63u) == 0) {
-      if (*reinterpret_cast<volatile int*>(err) != 0) return false;
+      if (!kSharedWord && *reinterpret_cast<volatile int*>(err) != 0) return false;
       if (global_ns() - t0 > limit) {
         atomicCAS(err, 0, site);
         return false;
@@ -89,8 +92,9 @@ TJ_DEV bool mbar_wait(uint64_t* bar, uint32_t parity, int* err, int site) {
 TJ_DEV bool error_raised(const int* err) { return *reinterpret_cast<const volatile int*>(err) != 0; }
 // Bounded wait executed by a whole warp; every lane gets the same answer, so
 // the warp stays converged for the elected tcgen05 issues that follow.
+template <bool kSharedWord = false>
 TJ_DEV bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* err, int site) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, site));
+  return __all_sync(0xffffffffu, mbar_wait<kSharedWord>(bar, parity, err, site));
 }
 // What a thread set going asynchronously is over before it goes on to leave
 // the kernel: it waits for its barriers' last phases, and where an expired wait

@@ -141,7 +141,7 @@ TJ_DEV bool mbar_wait_cluster_warp(uint64_t* bar, uint32_t parity, int* err, int
     return ok != 0;
   };
   if (__all_sync(0xffffffffu, try_wait())) return true;
-  if (!mbar_wait_warp(bar, parity, err, site)) return false;
+  if (!mbar_wait_warp<true>(bar, parity, err, site)) return false;
   return __all_sync(0xffffffffu, try_wait());  // complete: returns at once, with the acquire
 }
 
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
       const int mt = (int)(t / n_tiles), nt = (int)(t % n_tiles);
       if (!tile_has_rows(p.mask, mt * kG8BM, p.M, lane)) continue;
       for (int kb = 0; kb < kblocks; ++kb) {
-        if (!mbar_wait_warp(empty + stage, phase ^ 1u, p.err, kErrGemm8Producer)) { ok = false; break; }
+        if (!mbar_wait_warp<true>(empty + stage, phase ^ 1u, p.err, kErrGemm8Producer)) { ok = false; break; }
         if (lane == 0) {
           uint8_t* sa = smem + stage * Cfg::kStageBytes;
           mbar_expect_tx(full + stage, Cfg::kStageBytes);
@@ -377,12 +377,12 @@ __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
       for (int kb = 0; kb < kblocks; ++kb) {
         const bool first = kb % kChunk == 0;
         if (first) {
-          if (!mbar_wait_warp(acc_empty + abuf, aphase ^ 1u, p.err, kErrGemm8Mma)) { ok = false; break; }
+          if (!mbar_wait_warp<true>(acc_empty + abuf, aphase ^ 1u, p.err, kErrGemm8Mma)) { ok = false; break; }
         }
         if ((kb & 3) == 0) {
-          if (!mbar_wait_warp(sf_full + slot, sphase, p.err, kErrGemm8Mma)) { ok = false; break; }
+          if (!mbar_wait_warp<true>(sf_full + slot, sphase, p.err, kErrGemm8Mma)) { ok = false; break; }
         }
-        if (!mbar_wait_warp(full + stage, phase, p.err, kErrGemm8Mma)) { ok = false; break; }
+        if (!mbar_wait_warp<true>(full + stage, phase, p.err, kErrGemm8Mma)) { ok = false; break; }
         tc_fence_after();
         const uint32_t sa = smem_u32(smem + stage * Cfg::kStageBytes);
         const uint32_t sb = sa + kG8BM * 128;
@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
       };
       for (int kb = 0; kb < kblocks; kb += 4) {
         fetch(kb);
-        if (!mbar_wait_warp(sf_empty + slot, sphase ^ 1u, p.err, kErrGemm8Scales)) { ok = false; break; }
+        if (!mbar_wait_warp<true>(sf_empty + slot, sphase ^ 1u, p.err, kErrGemm8Scales)) { ok = false; break; }
         tc_fence_after();
         const uint32_t at = tmem_base + lanes + Cfg::kSfCol0 + slot * Cfg::kSfCols;
         tmem_st_words<4>(at, a);
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
       const bool valid = row < p.M && (p.mask == nullptr || __ldg(p.mask + row) != 0);
       const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + cg * Cfg::kCW;
       auto wait_acc = [&] {
-        ok = mbar_wait_warp(acc_full + abuf, aphase, p.err, kErrGemm8Epilogue);
+        ok = mbar_wait_warp<true>(acc_full + abuf, aphase, p.err, kErrGemm8Epilogue);
         tc_fence_after();
         return ok;
       };
@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
             uint8_t* buf = bufs + b * 4096;
             if (fetch) {
               uint64_t* bar = res_full + ew * Cfg::kBufs + b;
-              if (!mbar_wait_warp(bar, (rphase >> b) & 1u, p.err, kErrGemm8Epilogue)) {
+              if (!mbar_wait_warp<true>(bar, (rphase >> b) & 1u, p.err, kErrGemm8Epilogue)) {
                 ok = false;
                 Drain().wait(bar, (rphase >> b) & 1u);
                 __syncwarp();
@@ -759,7 +759,7 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
         if (!pair_has_rows(mt)) continue;
         if (lane == 0) {
           for (int kb = 0; kb < kblocks; ++kb) {
-            if (!mbar_wait(empty + stage, phase ^ 1u, p.err, kErrGemm8Producer)) { ok = false; break; }
+            if (!mbar_wait<true>(empty + stage, phase ^ 1u, p.err, kErrGemm8Producer)) { ok = false; break; }
             uint8_t* sa = smem + stage * Cfg::kStageBytes;
             const uint32_t lb = pair_leader_bar(full + stage);
             if (rank == 0) mbar_expect_tx(full + stage, 2 * Cfg::kStageBytes);
@@ -782,17 +782,17 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
         for (int kb = 0; kb < kblocks; ++kb) {
           const bool first = kb % kChunk == 0;
           if (first) {
-            if (!mbar_wait_warp(acc_empty + abuf, aphase ^ 1u, p.err, kErrGemm8Mma)) { ok = false; break; }
+            if (!mbar_wait_warp<true>(acc_empty + abuf, aphase ^ 1u, p.err, kErrGemm8Mma)) { ok = false; break; }
             if (any) {  // the accumulator before this one has given up the shared columns
-              if (!mbar_wait_warp(shared_free, shphase, p.err, kErrGemm8Mma)) { ok = false; break; }
+              if (!mbar_wait_warp<true>(shared_free, shphase, p.err, kErrGemm8Mma)) { ok = false; break; }
               shphase ^= 1u;
             }
             any = true;
           }
           if ((kb & 3) == 0) {
-            if (!mbar_wait_warp(sf_full + slot, sphase, p.err, kErrGemm8Mma)) { ok = false; break; }
+            if (!mbar_wait_warp<true>(sf_full + slot, sphase, p.err, kErrGemm8Mma)) { ok = false; break; }
           }
-          if (!mbar_wait_warp(full + stage, phase, p.err, kErrGemm8Mma)) { ok = false; break; }
+          if (!mbar_wait_warp<true>(full + stage, phase, p.err, kErrGemm8Mma)) { ok = false; break; }
           tc_fence_after();
           const uint32_t sa = smem_u32(smem + stage * Cfg::kStageBytes);
           const uint32_t sfa = tmem_base + Cfg::kSfCol0 + slot * Cfg::kSfCols;
@@ -855,7 +855,7 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
         const uint32_t wb[8] = {b0, b0, b0, b0, b4, b4, b4, b4};
         if (kb + 4 < kblocks) fetch(t, kb + 4);
         else fetch(after, 0);
-        if (!mbar_wait_warp(sf_empty + slot, sphase ^ 1u, p.err, kErrGemm8Scales)) { ok = false; break; }
+        if (!mbar_wait_warp<true>(sf_empty + slot, sphase ^ 1u, p.err, kErrGemm8Scales)) { ok = false; break; }
         tc_fence_after();
         const uint32_t at = tmem_base + lanes + Cfg::kSfCol0 + slot * Cfg::kSfCols;
         tmem_st_words<4>(at, wa);
@@ -893,7 +893,7 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
       const int row = row0 + lane;
       const bool valid = row < p.M && (p.mask == nullptr || __ldg(p.mask + row) != 0);
       auto wait_acc = [&] {
-        ok = mbar_wait_warp(acc_full + abuf, aphase, p.err, kErrGemm8Epilogue);
+        ok = mbar_wait_warp<true>(acc_full + abuf, aphase, p.err, kErrGemm8Epilogue);
         tc_fence_after();
         return ok;
       };
@@ -1025,7 +1025,7 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
             uint8_t* buf = bufs + b * 4096;
             if (fetch) {
               uint64_t* bar = res_full + 2 * ew + b;
-              if (!mbar_wait_warp(bar, (rphase >> b) & 1u, p.err, kErrGemm8Epilogue)) {
+              if (!mbar_wait_warp<true>(bar, (rphase >> b) & 1u, p.err, kErrGemm8Epilogue)) {
                 ok = false;
                 Drain().wait(bar, (rphase >> b) & 1u);
                 __syncwarp();

@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
         for (int s = im.s0; s < im.s1; ++s) {
           const int entry = p.list != nullptr ? p.list[s] : s;
           const int t0 = (entry & 0x7fffffff) * kWgTok;
-          if (!mbar_wait(empty + stage, phase ^ 1u, p.err, kErrWgradProducer)) { ok = false; break; }
+          if (!mbar_wait<true>(empty + stage, phase ^ 1u, p.err, kErrWgradProducer)) { ok = false; break; }
           uint8_t* sa = smem + stage * kWgStageBytes;
           const int k0 = im.k0 + (int)rank * 128;
           if (entry < 0) {
@@ -247,12 +247,12 @@ __global__ void __launch_bounds__(kWgThreads, 1)
         for (int s = im.s0; s < im.s1; ++s) {
           const bool first = (s - im.s0) % kWgChunk == 0;
           const int next = p.list != nullptr && s + 1 < im.s1 ? p.list[s + 1] : 0;
-          if (first && !mbar_wait_warp(acc_empty + abuf, aphase ^ 1u, p.err, kErrWgradMma)) { ok = false; break; }
+          if (first && !mbar_wait_warp<true>(acc_empty + abuf, aphase ^ 1u, p.err, kErrWgradMma)) { ok = false; break; }
           if (entry < 0) {
             if (!mbar_wait_cluster_warp(cleared + stage, (cbits >> stage) & 1u, p.err, kErrWgradMma)) { ok = false; break; }
             cbits ^= 1u << stage;
           } else {
-            if (!mbar_wait_warp(full + stage, (fbits >> stage) & 1u, p.err, kErrWgradMma)) { ok = false; break; }
+            if (!mbar_wait_warp<true>(full + stage, (fbits >> stage) & 1u, p.err, kErrWgradMma)) { ok = false; break; }
             fbits ^= 1u << stage;
           }
           entry = next;
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
               const long long t = t0 + 32 * h + lane;
               out[h] = __ballot_sync(0xffffffffu, t < p.T && __ldg(p.mask + t) == 0);
             }
-            if (!mbar_wait_warp(a_full + stage, (abits >> stage) & 1u, p.err, kErrWgradEdge)) { ok = false; break; }
+            if (!mbar_wait_warp<true>(a_full + stage, (abits >> stage) & 1u, p.err, kErrWgradEdge)) { ok = false; break; }
             abits ^= 1u << stage;
             uint8_t* sa = smem + stage * kWgStageBytes;
 #pragma unroll
@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
 #pragma unroll
       for (int q = 0; q < 128; ++q) acc[q] = 0.f;
       for (int s = im.s0; s < im.s1; s += kWgChunk) {
-        if (!mbar_wait_warp(acc_full + abuf, aphase, p.err, kErrWgradEpilogue)) { ok = false; break; }
+        if (!mbar_wait_warp<true>(acc_full + abuf, aphase, p.err, kErrWgradEpilogue)) { ok = false; break; }
         tc_fence_after();
         const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + abuf * 256 + half * 128;
 #pragma unroll

@@ -49,3 +49,34 @@ def test_expired_wait_leaves_in_order(m, n):
     # 262144 * 2^-18, exact in the accumulator
     assert torch.all(ops.gemm8(a, w, out_dtype=torch.bfloat16, err=err) == 1)
     assert int(err) == 0
+
+
+def test_earlier_error_ends_no_later_call():
+    """A word that holds an earlier call's site, the device's own or a caller's:
+    the products and the weight gradient run to their end all the same, and the
+    word keeps its site until it is read."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    rnd = lambda *s: torch.randn(*s, generator=g, device=DEV)
+    for m, n, k in ((300, 1024, 512), (3000, 2048, 640)):
+        a, w, bias, resid = ops.checkpoint8(rnd(m, k)), ops.pack_weight8(rnd(n, k)), rnd(n), rnd(m, n)
+        dy, x = rnd(m, n).bfloat16(), ops.checkpoint8(rnd(m, k))
+        word = torch.zeros(1, dtype=torch.int32, device=DEV)
+
+        def calls(err):
+            out = [ops.gemm8(a, w, bias, out_dtype=t, err=err) for t in (torch.float16, torch.bfloat16)]
+            out.append(ops.gemm8(a, w, bias, resid=resid, out_dtype=torch.float32, err=err))
+            for t in ops.gemm8_gelu(a, w, bias, err=err):
+                out += [t.codes.view(torch.uint8), t.scales.view(torch.uint8)]
+            return out + list(ops.linear_wgrad(dy, x, err=err))
+
+        want = calls(word)
+        assert int(word) == 0
+        word.fill_(403)
+        for got, exp in zip(calls(word), want):
+            assert torch.equal(got, exp)
+        assert int(word) == 403
+        own = ops._err_word(torch.cuda.current_device())
+        own.fill_(502)
+        for got, exp in zip(calls(None), want):
+            assert torch.equal(got, exp)
+        assert ops.device_error() == 502 and ops.device_error() == 0
