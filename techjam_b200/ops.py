@@ -15,6 +15,7 @@ nothing in sums.  Gradients are returned, not accumulated into anything.
 from __future__ import annotations
 
 import ctypes
+import threading
 from typing import NamedTuple, Optional
 
 import torch
@@ -290,19 +291,33 @@ def _err_ptr(err: Optional[torch.Tensor], index: int) -> int:
     return err.data_ptr()
 
 
+_err_lock = threading.Lock()
+_err_log: dict = {}            # device index: every site read from its word so far
+_err_seen = threading.local()  # per thread and device: how much of the log it has been told
+
+
 def device_error(device=None) -> int:
-    """Read (synchronously) and clear the error word that gemm8, gemm8_gelu and
+    """Read (synchronously) the error word that gemm8, gemm8_gelu and
     linear_wgrad share on a device: 0, or the site of the first bounded wait
-    that expired since the last call (their results since then are void)."""
+    that expired since this thread's last call (the results of the call that
+    waited are void, later ones are not affected).  Reading clears the word for
+    the kernels to come, not for other threads: each is told."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
-    torch.cuda.synchronize(device)
-    word = _err_word(device.index)
-    code = int(word.item())
-    if code:
-        word.zero_()
-    return code
+    with _err_lock:
+        word = _err_word(device.index)
+        torch.cuda.synchronize(device)
+        code = int(word.item())
+        log = _err_log.setdefault(device.index, [])
+        if code:
+            log.append(code)
+            word.zero_()
+            torch.cuda.synchronize(device)  # zero before a call on any other stream can set it again
+        seen = _err_seen.__dict__.setdefault("count", {})
+        new = log[seen.get(device.index, 0):]
+        seen[device.index] = len(log)
+    return new[0] if new else 0
 
 
 def checkpoint8(x: torch.Tensor, mask: Optional[torch.Tensor] = None) -> Act8:
