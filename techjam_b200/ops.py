@@ -204,10 +204,19 @@ class LayerNormOut(NamedTuple):
     x8: Optional[Act8]    # 8-bit copy of the input, when asked for
 
 
-_E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+# what a torch that lacks them needs only for the operators below (e8m0: from 2.7 on)
+_E4M3, _E8M0 = getattr(torch, "float8_e4m3fn", None), getattr(torch, "float8_e8m0fnu", None)
 # the handle and the index alone: the public forms build objects on each call
-_stream_of, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _entries: dict = {}
+
+
+def _need_8_bits():
+    if _E4M3 is None or _E8M0 is None:
+        raise RuntimeError(f"8-bit tensors need torch.float8_e4m3fn and torch.float8_e8m0fnu, which torch "
+                           f"{torch.__version__} lacks")
 
 
 def _run(index: int, name: str, *args) -> None:
@@ -255,6 +264,7 @@ def _blocks(n: int) -> int:
 
 def _check_act(a: Act8, what: str, index: Optional[int] = None):
     """Check an 8-bit activation; (device index, rows, cols)."""
+    _need_8_bits()
     if not isinstance(a, Act8):
         raise ValueError(f"{what} must be an Act8")
     index = _matrix(a.codes, what, (_E4M3,), None, index)
@@ -264,6 +274,7 @@ def _check_act(a: Act8, what: str, index: Optional[int] = None):
 
 
 def _new_act(rows: int, cols: int, device, dtype) -> Act8:
+    _need_8_bits()
     return Act8(torch.empty(rows, cols, dtype=_E4M3, device=device),
                 torch.empty(rows, _blocks(cols), dtype=_E8M0, device=device), dtype)
 
@@ -347,6 +358,7 @@ def restore8(a: Act8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
 def pack_weight8(w: torch.Tensor, transpose: bool = False) -> Weight8:
     """A weight [n, k] (fp32, fp16 or bf16) into 8 bits, or its transpose (for
     the product that takes a gradient back through the layer)."""
+    _need_8_bits()
     index = _matrix(w, "w", _DTYPES)
     n, k = w.shape
     if not 0 < n < _MAX:
@@ -371,7 +383,7 @@ def layernorm_train(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor, m
     _matrix(bias, "bias", _F32, (d,), index)
     mptr = _row_mask(mask, rows, index)
     dev = x.device
-    if out_dtype == _E4M3:
+    if out_dtype == _E4M3 and out_dtype is not None:
         y = _new_act(rows, d, dev, x.dtype)
         yp, ys, yd = y.codes.data_ptr(), y.scales.data_ptr(), _lib.E4M3
     elif out_dtype in _DTYPES:

@@ -1,11 +1,15 @@
 """Host-side bookkeeping of the training and 8-bit operators, without a GPU."""
 
+import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import torch
 
 from techjam_b200 import ops
 
+ROOT = Path(__file__).resolve().parent.parent
 
 class Word:
     """A device's error word: counts as zeroed only once the device was waited for."""
@@ -47,3 +51,32 @@ def test_device_error_is_told_to_every_thread(monkeypatch):
     assert ops.device_error("cuda:0") == 0
     assert elsewhere() == (402, 0)  # a thread that has never asked: all since the start, the first of them
     assert ops.device_error("cuda:1") == 0
+
+
+LEAN = """
+import torch
+for owner, name in ((torch, "float8_e4m3fn"), (torch, "float8_e8m0fnu"), (torch._C, "_cuda_getCurrentRawStream"),
+                    (torch._C, "_cuda_getDevice")):
+    if hasattr(owner, name):
+        delattr(owner, name)
+from techjam_b200 import ops
+assert callable(ops.layernorm) and callable(ops.gemm) and callable(ops.attention)
+assert callable(ops._stream_of) and callable(ops._current_device)
+a = ops.Act8(torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(4, 1, dtype=torch.uint8), torch.float32)
+w = torch.zeros(64, 64)
+for call in (lambda: ops.restore8(a), lambda: ops.pack_weight8(w), lambda: ops._new_act(4, 64, "cpu", torch.float32),
+             lambda: ops.gemm8(a, ops.Weight8(w, w))):
+    try:
+        call()
+    except RuntimeError as e:
+        assert "float8" in str(e)
+    else:
+        raise AssertionError("not refused")
+print("fine")
+"""
+
+
+def test_a_torch_without_8_bit_types_keeps_the_other_operators():
+    """The 8-bit operators say what they lack; the module and the operators of before do without."""
+    got = subprocess.run([sys.executable, "-c", LEAN], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0 and got.stdout.strip().endswith("fine"), got.stderr
