@@ -146,6 +146,7 @@ int tj_layernorm_backward(const void* dy, int dy_dtype, const void* x, const uin
   if (!plain(dy_dtype) || !plain(dx_dtype)) return fail(TJ_ERR_INVALID, "unknown dtype");
   if (!gamma || !dgamma || !dbeta || (rows > 0 && (!dy || !x || !mean || !rstd || !dx)))
     return fail(TJ_ERR_INVALID, "null argument");
+  if (!aligned(workspace, 4)) return fail(TJ_ERR_INVALID, "workspace not 4-byte aligned");
   size_t need = 0;
   TJH_CHECK(tj_layernorm_backward_workspace_bytes(rows, d, &need));
   if (workspace_bytes < need || (need > 0 && !workspace))

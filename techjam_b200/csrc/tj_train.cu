@@ -24,13 +24,13 @@ bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) &
 bool plain(int dtype) { return dtype == TJ_F32 || dtype == TJ_F16 || dtype == TJ_BF16; }
 size_t vec_bytes(int dtype) { return dtype == TJ_F32 ? 16 : 8; }
 int blocks_of(int cols) { return (cols + tj::kBlk - 1) / tj::kBlk; }
+constexpr int kMaxSize = 0x7fffff00;  // sizes up to here can be rounded up to a tile in an int
 
 // CTAs for 8 lanes per 128-column block, 256 threads each.
 int block_grid(long long rows, int cols, unsigned* grid) {
   if (rows < 0 || cols <= 0) return fail(TJ_ERR_INVALID, "rows %lld, columns %d", rows, cols);
-  const long long ctas = (rows * blocks_of(cols) + 31) / 32;
-  if (ctas > 0x7fffffffLL) return fail(TJ_ERR_UNSUPPORTED, "too many blocks");
-  *grid = (unsigned)ctas;
+  if (cols > kMaxSize || rows > 0x7fffffffLL * 32 / blocks_of(cols)) return fail(TJ_ERR_UNSUPPORTED, "too many blocks");
+  *grid = (unsigned)((rows * blocks_of(cols) + 31) / 32);
   return TJ_OK;
 }
 
@@ -186,7 +186,7 @@ int launch_gemm8_pair(const Gemm8Args& g, const tj::Gemm8Params& p, int dev, cud
 int gemm8_params(tj::Gemm8Params* p, const void* a, const uint8_t* as, const void* w, const uint8_t* ws,
                  const float* bias, int m, int n, int k, const uint8_t* mask, int* err) {
   if (m < 0 || n <= 0 || k <= 0) return fail(TJ_ERR_INVALID, "product of [%d, %d] and [%d, %d]", m, k, n, k);
-  if (m > 0x7fffff00 || n > 0x7fffff00 || k > 0x7fffff00) return fail(TJ_ERR_UNSUPPORTED, "product too large");
+  if (m > kMaxSize || n > kMaxSize || k > kMaxSize) return fail(TJ_ERR_UNSUPPORTED, "product too large");
   if (!w || !ws || !err || (m > 0 && (!a || !as))) return fail(TJ_ERR_INVALID, "null argument");
   if (k % 16) return fail(TJ_ERR_UNSUPPORTED, "need k %% 16 == 0");
   if (bias != nullptr && !aligned(bias, 16)) return fail(TJ_ERR_INVALID, "bias not 16-byte aligned");
@@ -221,7 +221,7 @@ struct WgradPlan {
 int wgrad_plan(long long rows, int n, int k, int sms, WgradPlan* w) {
   if (rows < 0 || n <= 0 || k <= 0) return fail(TJ_ERR_INVALID, "weight gradient of [%lld, %d] and [%lld, %d]", rows, n, rows, k);
   if (n % 8 || k % 16) return fail(TJ_ERR_UNSUPPORTED, "need n %% 8 == 0 and k %% 16 == 0");
-  if (rows > 0x7fffffffLL) return fail(TJ_ERR_UNSUPPORTED, "too many rows");
+  if (rows > 0x7fffffffLL || n > kMaxSize || k > kMaxSize) return fail(TJ_ERR_UNSUPPORTED, "weight gradient too large");
   const long long stages = (rows + tj::kWgTok - 1) / tj::kWgTok;
   w->k_tiles = (k + 255) / 256;
   const long long tiles = (long long)((n + 255) / 256) * w->k_tiles;
@@ -298,8 +298,8 @@ int tj_weight8_pack(const void* w, int dtype, int n, int k, int transpose, void*
   if (n <= 0 || k <= 0) return fail(TJ_ERR_INVALID, "weight [%d, %d]", n, k);
   if (!plain(dtype)) return fail(TJ_ERR_INVALID, "unknown dtype %d", dtype);
   if (!w || !codes || !scales) return fail(TJ_ERR_INVALID, "null argument");
+  if (k > kMaxSize || n > 65535 * tj::kBlk) return fail(TJ_ERR_UNSUPPORTED, "weight [%d, %d] too large", n, k);
   const dim3 grid(blocks_of(k), blocks_of(n));
-  if (grid.y > 65535) return fail(TJ_ERR_UNSUPPORTED, "too many rows");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint8_t* c = static_cast<uint8_t*>(codes);
 #define TJ_WPACK(T)                                                                                                  \

@@ -5,10 +5,12 @@ import sys
 import threading
 from pathlib import Path
 
+import pytest
 import torch
 
-from techjam_b200 import ops
+from techjam_b200 import _lib, build, ops
 
+INVALID, UNSUPPORTED = 1, 2
 ROOT = Path(__file__).resolve().parent.parent
 
 class Word:
@@ -54,12 +56,13 @@ def test_device_error_is_told_to_every_thread(monkeypatch):
 
 
 LEAN = """
+import pytest
 import torch
 for owner, name in ((torch, "float8_e4m3fn"), (torch, "float8_e8m0fnu"), (torch._C, "_cuda_getCurrentRawStream"),
                     (torch._C, "_cuda_getDevice")):
     if hasattr(owner, name):
         delattr(owner, name)
-from techjam_b200 import ops
+from techjam_b200 import _lib, build, ops
 assert callable(ops.layernorm) and callable(ops.gemm) and callable(ops.attention)
 assert callable(ops._stream_of) and callable(ops._current_device)
 a = ops.Act8(torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(4, 1, dtype=torch.uint8), torch.float32)
@@ -80,3 +83,26 @@ def test_a_torch_without_8_bit_types_keeps_the_other_operators():
     """The 8-bit operators say what they lack; the module and the operators of before do without."""
     got = subprocess.run([sys.executable, "-c", LEAN], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert got.returncode == 0 and got.stdout.strip().endswith("fine"), got.stderr
+
+
+BIG = 0x7fffffff
+P = 1 << 20  # a non-null, 16-byte aligned pointer that no refused call reads
+
+
+@pytest.mark.parametrize("name,args,want", [
+    # sizes that cannot be rounded up to a block or a tile in an int, or whose count of blocks passes 64 bits
+    ("tj_act8_pack", (P, 0, 1, BIG, None, P, P, None), UNSUPPORTED),
+    ("tj_act8_pack", (P, 0, 1 << 62, 4096, None, P, P, None), UNSUPPORTED),
+    ("tj_act8_unpack", (P, P, 1, BIG, P, 0, None), UNSUPPORTED),
+    ("tj_gelu_backward", (P, 0, P, None, 1, BIG, None, P, None, None, None), UNSUPPORTED),
+    ("tj_weight8_pack", (P, 0, BIG, 4, 0, P, P, None), UNSUPPORTED),
+    ("tj_weight8_pack", (P, 0, 4, BIG, 0, P, P, None), UNSUPPORTED),
+    ("tj_weight8_pack", (P, 0, 65535 * 128 + 1, 4, 0, P, P, None), UNSUPPORTED),
+    ("tj_gemm8", (P, P, P, P, None, 4, BIG - 7, 32, None, None, P, 0, P, None), UNSUPPORTED),
+    # the workspace holds floats
+    ("tj_layernorm_backward", (P, 0, P, None, P, P, P, 4, 64, None, None, P, 0, P, P, P + 2, 1 << 20, None), INVALID),
+])
+def test_c_entries_refuse_sizes_and_alignment(name, args, want):
+    build.build()
+    assert getattr(_lib.load(), name)(*args) == want
+    assert _lib.load().tj_last_error()
