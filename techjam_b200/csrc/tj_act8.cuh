@@ -306,8 +306,10 @@ __global__ void __launch_bounds__(256) act8_unpack_kernel(const uint8_t* __restr
 }
 
 // One CTA per 128 x 128 block of a weight [n, k]: codes [n, k] (or [k, n]
-// when TR) and one scale per block.  Runs when weights are loaded, not per
-// step; the transposed copy goes through shared memory.
+// when TR) and one scale per block; the transposed copy goes through shared
+// memory.  A model that serves packs once, one that trains packs both orders
+// every step.  Two passes over the block in single elements, the second from
+// L1 and L2: 18 us for 4096 x 1024 fp32, 22 transposed, where its 21 MB take 3.
 template <typename T, bool TR>
 __global__ void __launch_bounds__(256) weight8_pack_kernel(const T* __restrict__ w, int n, int k,
                                                            uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {

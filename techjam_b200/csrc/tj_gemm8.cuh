@@ -671,7 +671,7 @@ struct Gemm8PairCfg {
   static constexpr int kSfSlots = 2;
   static constexpr int kSfCols = 12;  // 4 for A's 128 rows, 8 for W's 256
   static constexpr int kThreads = 256 + 32 * kEpiWarps;
-  // kG8Gelu: warpgroups with 24 + 40 + 4 * 104 (96: 55 us for 47); kG8F32: 56 + 56 + 2 * 200
+  // kG8Gelu: warpgroups with 24 + 40 + 4 * 104 (96 spilled more and took a sixth longer); kG8F32: 56 + 56 + 2 * 200
   static constexpr int kRegLaunch = KIND == kG8Gelu ? 80 : 128;
   static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kStagingBytes + 512;
   static_assert(kSmemBytes <= 232448, "shared memory");

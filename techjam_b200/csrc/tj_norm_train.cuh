@@ -75,7 +75,9 @@ struct NormFwdParams {
 // CTAs per SM forward.  What hides the loads is rows in flight: 32768 x 1024
 // fp32 to fp16, padded, took 41, 35 and 32 us with 4, 6 and 8; packing and the
 // scalar loads need the registers of 6 (48 us to 8 bits with a copy of x, 49
-// with 8).
+// with 8).  To 8 bits with a copy of x the ALU pipe, which takes packing's
+// maxima and conversions, is busy 64% of the time and 69% of the issue slots
+// are taken, at 3.3 TB/s.
 template <typename Y>
 constexpr int norm_fwd_ctas(bool vec) { return std::is_same_v<Y, uint8_t> || !vec ? 6 : 8; }
 
@@ -164,29 +166,28 @@ struct NormBwdParams {
 
 // DY: type of dy; X: type of dx (and of x unless X8).  A CTA walks rows with
 // a stride; each lane keeps the sums of its own columns, joined over the
-// CTA's row groups at the end and over the CTAs by norm_grad_kernel, always
-// in the same order.
+// CTA's row groups at the end and over the CTAs by column_sum_kernel, always
+// in the same order.  What bounds it is the latency of a row's loads with 16
+// warps an SM: with an 8-bit x 7 of the 10.8 cycles between a warp's
+// instructions wait for global memory, at 4.5 TB/s (32768 x 1024, 76 us).
 template <typename DY, typename X, bool X8, int WR, bool VEC>
 __global__ void __launch_bounds__(32 * norm_bwd_warps(WR), norm_bwd_ctas(WR)) norm_bwd_kernel(const NormBwdParams p) {
-  constexpr int NI = 1;
   constexpr int kWarps = norm_bwd_warps(WR);
   constexpr int kGroups = kWarps / WR;  // rows in flight per CTA
   __shared__ float s_red[2][kWarps * 2];
   int red = 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int base = (warp % WR) * 512;
+  // the lane's block: of the warp's 512 columns, and of the row
+  const int blk = norm_blk(lane, 0), c0 = (warp % WR) * 512 + blk, sub = lane & 7;
   const int d = p.d, nb = n_blocks(d);
   const float inv_d = 1.f / d;
-  float acc_w[NI][4][4], acc_b[NI][4][4];
+  float acc_w[4][4], acc_b[4][4];
 #pragma unroll
-  for (int i = 0; i < NI; ++i)
+  for (int j = 0; j < 4; ++j)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc_w[i][j][e] = acc_b[i][j][e] = 0.f;
+    for (int e = 0; e < 4; ++e) acc_w[j][e] = acc_b[j][e] = 0.f;
 
   const long long step = (long long)gridDim.x * kGroups;
-  const int sub = lane & 7;
   auto valid_at = [&](long long row) { return row < p.rows && (p.mask == nullptr || p.mask[row] != 0); };
   bool valid = valid_at((long long)blockIdx.x * kGroups + warp / WR);
   // the CTA's row groups run the same number of iterations: row_sum meets at barriers
@@ -197,76 +198,57 @@ __global__ void __launch_bounds__(32 * norm_bwd_warps(WR), norm_bwd_ctas(WR)) no
     const long long at = in ? row * d : 0;
     // everything that the row needs is on its way before anything waits
     const float mean = valid ? p.mean[row] : 0.f, rstd = valid ? p.rstd[row] : 0.f;
-    float g[NI][4][4], xh[NI][4][4], r[NI][4][4];
+    float g[4][4], xh[4][4], r[4][4];
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
+    for (int j = 0; j < 4; ++j) load4<DY, VEC>(static_cast<const DY*>(p.dy) + at, c0, sub, j, lim, g[j]);
+    if constexpr (X8) {
+      const float s = c0 < lim ? scale_value(p.x_scales[row * nb + c0 / kBlk]) : 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        load4<DY, VEC>(static_cast<const DY*>(p.dy) + at, base + norm_blk(lane, i), sub, j, lim, g[i][j]);
-    if constexpr (X8) {
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int c0 = base + norm_blk(lane, i);
-        const float s = c0 < lim ? scale_value(p.x_scales[row * nb + c0 / kBlk]) : 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          e4m3x4_value(load_codes4<VEC>(static_cast<const uint8_t*>(p.x) + at, c0, sub, j, lim), s, xh[i][j]);
-      }
+        e4m3x4_value(load_codes4<VEC>(static_cast<const uint8_t*>(p.x) + at, c0, sub, j, lim), s, xh[j]);
     } else {
 #pragma unroll
-      for (int i = 0; i < NI; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          load4<X, VEC>(static_cast<const X*>(p.x) + at, base + norm_blk(lane, i), sub, j, lim, xh[i][j]);
+      for (int j = 0; j < 4; ++j) load4<X, VEC>(static_cast<const X*>(p.x) + at, c0, sub, j, lim, xh[j]);
     }
     if (p.resid != nullptr) {
 #pragma unroll
-      for (int i = 0; i < NI; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          load4<X, VEC>(static_cast<const X*>(p.resid) + at, base + norm_blk(lane, i), sub, j, lim, r[i][j]);
+      for (int j = 0; j < 4; ++j) load4<X, VEC>(static_cast<const X*>(p.resid) + at, c0, sub, j, lim, r[j]);
     } else {
 #pragma unroll
-      for (int i = 0; i < NI; ++i)
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) r[i][j][e] = 0.f;
+        for (int e = 0; e < 4; ++e) r[j][e] = 0.f;
     }
     const bool valid_next = valid_at(row + step);
     float s[2] = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
+    for (int j = 0; j < 4; ++j) {
+      float gm[4];
+      load4<float, VEC>(p.gamma, c0, sub, j, d, gm);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float gm[4];
-        load4<float, VEC>(p.gamma, base + norm_blk(lane, i), sub, j, d, gm);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float xv = valid ? (xh[i][j][e] - mean) * rstd : 0.f;
-          const float dyv = g[i][j][e];  // 0 past the row's end and for masked rows
-          acc_w[i][j][e] += dyv * xv;
-          acc_b[i][j][e] += dyv;
-          const float gv = dyv * gm[e];
-          s[0] += gv;
-          s[1] += gv * xv;
-          xh[i][j][e] = xv;
-          g[i][j][e] = gv;
-        }
+      for (int e = 0; e < 4; ++e) {
+        const float xv = valid ? (xh[j][e] - mean) * rstd : 0.f;
+        const float dyv = g[j][e];  // 0 past the row's end and for masked rows
+        acc_w[j][e] += dyv * xv;
+        acc_b[j][e] += dyv;
+        const float gv = dyv * gm[e];
+        s[0] += gv;
+        s[1] += gv * xv;
+        xh[j][e] = xv;
+        g[j][e] = gv;
       }
+    }
     row_sum<kWarps, WR, 2>(s, s_red, red, warp, lane);
     const float m0 = s[0] * inv_d, m1 = s[1] * inv_d;
     if (in) {
 #pragma unroll
-      for (int i = 0; i < NI; ++i)
+      for (int j = 0; j < 4; ++j) {
+        X o[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          X o[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            o[e] = from_f32<X>(valid ? rstd * (g[i][j][e] - m0 - xh[i][j][e] * m1) + r[i][j][e] : 0.f);
-          store4<X, VEC>(static_cast<X*>(p.dx) + at, base + norm_blk(lane, i), sub, j, d, o);
-        }
+        for (int e = 0; e < 4; ++e)
+          o[e] = from_f32<X>(valid ? rstd * (g[j][e] - m0 - xh[j][e] * m1) + r[j][e] : 0.f);
+        store4<X, VEC>(static_cast<X*>(p.dx) + at, c0, sub, j, d, o);
+      }
     }
     valid = valid_next;
   }
@@ -286,32 +268,26 @@ __global__ void __launch_bounds__(32 * norm_bwd_warps(WR), norm_bwd_ctas(WR)) no
           __syncthreads();
           if (warp / WR == w && warp % WR == half)
 #pragma unroll
-            for (int i = 0; i < NI; ++i)
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s_acc[norm_col<VEC>(lane, i, j, e)] = acc[i][j][e];
+              for (int e = 0; e < 4; ++e) s_acc[piece_col<VEC>(blk, sub, j, e)] = acc[j][e];
           __syncthreads();
           if (warp / WR == 0 && warp % WR == half)
 #pragma unroll
-            for (int i = 0; i < NI; ++i)
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] += s_acc[norm_col<VEC>(lane, i, j, e)];
+              for (int e = 0; e < 4; ++e) acc[j][e] += s_acc[piece_col<VEC>(blk, sub, j, e)];
         }
       }
     }
     if (warp / WR == 0)
 #pragma unroll
-      for (int i = 0; i < NI; ++i)
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int c = base + norm_col<VEC>(lane, i, j, e);
-            if (c < d) out[c] = acc[i][j][e];
-          }
+        for (int e = 0; e < 4; ++e) {
+          const int c = piece_col<VEC>(c0, sub, j, e);
+          if (c < d) out[c] = acc[j][e];
+        }
   }
 }
 
