@@ -366,6 +366,7 @@ __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
       }
     }
     if (lane == 0) Drain().ring(full, S, stage, phase);
+    __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     int stage = 0, abuf = 0, slot = 0;
@@ -638,6 +639,7 @@ __global__ void __launch_bounds__(Gemm8Cfg<BN, KIND>::kThreads, 1)
       }
     }
     if (lane == 0) bulk_wait_all();
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
@@ -772,6 +774,7 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
       }
       // the loads signal the even CTA, but both learn when the MMAs have used them
       if (lane == 0) Drain().ring(empty, S, stage, phase);
+      __syncwarp();
     } else if (warp == 1 && rank == 0) {
       // ---------------------------------------------------------- MMA issuer
       int stage = 0, abuf = 0, slot = 0;
@@ -1112,6 +1115,7 @@ __global__ void __launch_bounds__(Gemm8PairCfg<KIND>::kThreads, 1)
       }
     }
     if (lane == 0) bulk_wait_all();
+    __syncwarp();
   }
   tc_fence_before();
   cluster_sync();

@@ -389,6 +389,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
       }
     }
   }
+  __syncwarp();  // the loading thread's warp too is whole again at the aligned barrier
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
